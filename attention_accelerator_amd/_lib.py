@@ -27,6 +27,9 @@ GQA_ROPE_K = 2
 GQA_PLAN_STREAM_K = 4
 GQA_PLAN_NO_MULTI_TOKEN = 8
 
+GQA_Q8_INT8 = 0
+GQA_Q8_E4M3 = 1
+
 # Every function include/gqa.h declares (checked by the CPU test suite).
 EXPORTS = (
     "gqa_validate_registers",
@@ -44,6 +47,10 @@ EXPORTS = (
     "gqa_prefill_bf16",
     "gqa_prefill_rescored_rows_offset",
     "gqa_kv_append_bf16",
+    "gqa_paged_plan",
+    "gqa_kv_append_q8",
+    "gqa_attention_q8_workspace_bytes",
+    "gqa_attention_q8",
     "gqa_rope_rows_bf16",
     "gqa_profile_enable",
     "gqa_profile_read",
@@ -82,6 +89,20 @@ class GqaPagedKv(ctypes.Structure):
         ("block_size", ctypes.c_int32),
         ("max_blocks", ctypes.c_int32),
         ("n_blocks", ctypes.c_int32),
+    ]
+
+
+class GqaQ8Kv(ctypes.Structure):
+    _fields_ = [
+        ("block_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+        ("pos_stride", ctypes.c_int64),
+        ("scale_block_stride", ctypes.c_int64),
+        ("scale_head_stride", ctypes.c_int64),
+        ("block_size", ctypes.c_int32),
+        ("max_blocks", ctypes.c_int32),
+        ("n_blocks", ctypes.c_int32),
+        ("format", ctypes.c_int32),
     ]
 
 
@@ -162,6 +183,17 @@ def lib() -> ctypes.CDLL:
                                      ctypes.POINTER(GqaKvLayout), vp, ctypes.c_int32, ctypes.c_int32,
                                      vp]
     L.gqa_kv_append_bf16.restype = ctypes.c_int
+    i32, i64 = ctypes.c_int32, ctypes.c_int64
+    L.gqa_paged_plan.argtypes = [vp, vp, i32, vp, vp, i32, vp, i64, i32, i32, vp, vp, vp, vp, vp, vp]
+    L.gqa_paged_plan.restype = ctypes.c_int
+    L.gqa_kv_append_q8.argtypes = [ctypes.POINTER(GqaParams), vp, i64, vp, i64, vp, vp, vp, vp,
+                                   ctypes.POINTER(GqaQ8Kv), vp, vp, i32, vp]
+    L.gqa_kv_append_q8.restype = ctypes.c_int
+    L.gqa_attention_q8_workspace_bytes.argtypes = [ctypes.POINTER(GqaParams), i32, i32, i32]
+    L.gqa_attention_q8_workspace_bytes.restype = ctypes.c_size_t
+    L.gqa_attention_q8.argtypes = [ctypes.POINTER(GqaParams), vp, i64, vp, vp, vp, vp, ctypes.POINTER(GqaQ8Kv),
+                                   vp, vp, vp, i32, i32, i32, vp, vp, ctypes.c_size_t, vp]
+    L.gqa_attention_q8.restype = ctypes.c_int
     L.gqa_rope_rows_bf16.argtypes = [vp, vp, ctypes.c_int64, ctypes.c_int64, vp, ctypes.c_int32,
                                      ctypes.c_double, vp]
     L.gqa_rope_rows_bf16.restype = ctypes.c_int

@@ -9,7 +9,8 @@ from pathlib import Path
 PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
-SOURCES = ("gqa_abi.hip", "gqa_decode.hip", "gqa_prefill.hip", "gqa_multitoken.hip", "gqa_rope.hip")
+SOURCES = ("gqa_abi.hip", "gqa_decode.hip", "gqa_prefill.hip", "gqa_multitoken.hip", "gqa_rope.hip",
+           "gqa_plan.hip", "gqa_q8_append.hip", "gqa_q8_attn.hip")
 OUT = PKG / "libgqa.so"
 
 HIPCC_FLAGS = [

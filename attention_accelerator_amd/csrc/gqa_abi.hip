@@ -11,6 +11,7 @@
 
 #include "gqa.h"
 #include "gqa_internal.h"
+#include "gqa_q8.h"
 
 namespace gqa {
 
@@ -749,6 +750,177 @@ int gqa_prefill_bf16(const gqa_params_t* params, const uint16_t* q, const uint16
         (void)hipEventRecord(ev[4], s);
     }
     return e == hipSuccess ? GQA_OK : GQA_ERR_HIP;
+}
+
+}  // extern "C"
+
+namespace {
+
+bool q8_layout_ok(const gqa_q8_kv_t* kv) {
+    return kv->block_size == 16 && kv->n_blocks > 0 && kv->n_blocks < (1 << 27) && kv->pos_stride >= kD &&
+           kv->pos_stride < (int64_t{1} << 27) && kv->head_stride >= 0 && kv->block_stride >= 0 &&
+           kv->scale_block_stride >= 0 && kv->scale_head_stride >= 0 &&
+           (kv->format == GQA_Q8_INT8 || kv->format == GQA_Q8_E4M3);
+}
+
+bool q8_pool_aligned(const gqa_q8_kv_t* kv, const void* k, const void* v, const void* ks, const void* vs) {
+    return aligned(k, 16) && aligned(v, 16) && aligned(ks, 4) && aligned(vs, 4) && kv->pos_stride % 16 == 0 &&
+           kv->head_stride % 16 == 0 && kv->block_stride % 16 == 0;
+}
+
+Q8Pool q8_pool(const gqa_q8_kv_t* kv, const void* k, const void* v, const float* ks, const float* vs) {
+    Q8Pool p{};
+    p.k = static_cast<const uint8_t*>(k);
+    p.v = static_cast<const uint8_t*>(v);
+    p.k_scale = ks;
+    p.v_scale = vs;
+    p.block_stride = kv->block_stride;
+    p.head_stride = kv->head_stride;
+    p.pos_stride = kv->pos_stride;
+    p.scale_block_stride = kv->scale_block_stride;
+    p.scale_head_stride = kv->scale_head_stride;
+    p.n_blocks = kv->n_blocks;
+    return p;
+}
+
+// Ranges of the stream kernel (one-wave workgroups) and workgroups of the tile kernel.
+int32_t q8_stream_waves(const gqa_params_t* p, int32_t max_new) {
+    const int32_t cus = stream_wgs(p) / kWavesPerCu;
+    return cus > 0 ? cus * q8_waves_per_cu(max_new) : 1;
+}
+
+int32_t q8_tile_wgs(const gqa_params_t* p) {
+    const int32_t cus = stream_wgs(p) / kWavesPerCu;
+    return cus > 0 ? cus * kQ8TileWgsPerCu : 1;
+}
+
+// Partial rows of the stream kernel (two pieces of every range), then of the tile kernel.
+int64_t q8_stream_rows(const gqa_params_t* p, int32_t max_new) {
+    return int64_t{2} * q8_stream_waves(p, max_new) * 16 * q8_stream_tiles(max_new);
+}
+
+int64_t q8_rows(const gqa_params_t* p, int32_t max_new) {
+    const int64_t tile = max_new > kQ8StreamMax ? static_cast<int64_t>(q8_tile_wgs(p)) * kQ8TileTokens * kGroup : 0;
+    return q8_stream_rows(p, max_new) + tile;
+}
+
+}  // namespace
+
+extern "C" {
+
+int gqa_paged_plan(const int32_t* cached, const int32_t* n_new, int32_t batch, const int32_t* free_blocks,
+                   const int32_t* n_free, int32_t free_capacity, int32_t* block_table, int64_t table_stride,
+                   int32_t max_blocks, int32_t n_rows, int32_t* seq_len, int32_t* cu_new, int32_t* slot_map,
+                   int32_t* positions, int32_t* n_free_out, void* stream) {
+    if (batch <= 0 || n_rows < 0 || free_capacity < 0 || max_blocks <= 0 || max_blocks > 0x7FFFFFF ||
+        table_stride < max_blocks)
+        return GQA_ERR_INVALID_CONFIG;
+    if (!cached || !n_new || !n_free || !block_table || !seq_len || !cu_new || !n_free_out) return GQA_ERR_BAD_POINTER;
+    if ((free_capacity > 0 && !free_blocks) || (n_rows > 0 && (!slot_map || !positions))) return GQA_ERR_BAD_POINTER;
+    for (const void* p : {static_cast<const void*>(cached), static_cast<const void*>(n_new),
+                          static_cast<const void*>(free_blocks), static_cast<const void*>(n_free),
+                          static_cast<const void*>(block_table), static_cast<const void*>(seq_len),
+                          static_cast<const void*>(cu_new), static_cast<const void*>(slot_map),
+                          static_cast<const void*>(positions), static_cast<const void*>(n_free_out)})
+        if (!aligned(p, 4)) return GQA_ERR_BAD_POINTER;
+    // Workgroups read the lengths while others write: an output that starts at an input races.
+    for (const void* p : {static_cast<const void*>(seq_len), static_cast<const void*>(cu_new),
+                          static_cast<const void*>(slot_map), static_cast<const void*>(positions),
+                          static_cast<const void*>(n_free_out)})
+        if (p && (p == cached || p == n_new || p == free_blocks || p == n_free)) return GQA_ERR_BAD_POINTER;
+    PagedPlanArgs a{};
+    a.cached = cached;
+    a.n_new = n_new;
+    a.free_blocks = free_blocks;
+    a.n_free = n_free;
+    a.block_table = block_table;
+    a.table_stride = table_stride;
+    a.seq_len = seq_len;
+    a.cu_new = cu_new;
+    a.slot_map = slot_map;
+    a.positions = positions;
+    a.n_free_out = n_free_out;
+    a.batch = batch;
+    a.max_blocks = max_blocks;
+    a.free_capacity = free_capacity;
+    a.n_rows = n_rows;
+    return launch_paged_plan(a, static_cast<hipStream_t>(stream)) == hipSuccess ? GQA_OK : GQA_ERR_HIP;
+}
+
+int gqa_kv_append_q8(const gqa_params_t* params, const uint16_t* k_new, int64_t k_token_stride,
+                     const uint16_t* v_new, int64_t v_token_stride, void* k_pool, void* v_pool, float* k_scale,
+                     float* v_scale, const gqa_q8_kv_t* kv, const int32_t* slots, const int32_t* positions,
+                     int32_t n_tokens, void* stream) {
+    if (!params || !kv) return GQA_ERR_BAD_POINTER;
+    if (!geometry_ok(params) || !q8_layout_ok(kv) || n_tokens < 0) return GQA_ERR_INVALID_CONFIG;
+    if (k_token_stride < 0 || v_token_stride < 0) return GQA_ERR_INVALID_CONFIG;
+    if (n_tokens == 0) return GQA_OK;
+    const bool rope = (params->flags & GQA_ROPE_K) != 0;
+    if (!k_new || !v_new || !k_pool || !v_pool || !k_scale || !v_scale || !slots || (rope && !positions))
+        return GQA_ERR_BAD_POINTER;
+    if (!aligned(k_new, 8) || !aligned(v_new, 8) || k_token_stride % 4 || v_token_stride % 4 || !aligned(slots, 4) ||
+        !aligned(positions, 4) || !q8_pool_aligned(kv, k_pool, v_pool, k_scale, v_scale))
+        return GQA_ERR_BAD_POINTER;
+    Q8AppendArgs a{};
+    a.pool = q8_pool(kv, k_pool, v_pool, k_scale, v_scale);
+    a.k_new = k_new;
+    a.v_new = v_new;
+    a.k_token_stride = k_token_stride;
+    a.v_token_stride = v_token_stride;
+    a.slots = slots;
+    a.positions = positions;
+    a.n_tokens = n_tokens;
+    a.rope = rope;
+    if (rope) fill_rope_table(params->rope_theta, &a.rope_table);
+    return launch_q8_append(a, kv->format, static_cast<hipStream_t>(stream)) == hipSuccess ? GQA_OK : GQA_ERR_HIP;
+}
+
+size_t gqa_attention_q8_workspace_bytes(const gqa_params_t* params, int32_t batch, int32_t n_tokens, int32_t max_new) {
+    if (!params || !geometry_ok(params) || batch <= 0 || n_tokens <= 0 || max_new <= 0) return 0;
+    const size_t rows = static_cast<size_t>(q8_rows(params, max_new));
+    return align_up(rows * kD * sizeof(float), 256) + align_up(rows * sizeof(float4), 256);
+}
+
+int gqa_attention_q8(const gqa_params_t* params, const uint16_t* q, int64_t q_token_stride, const void* k_pool,
+                     const void* v_pool, const float* k_scale, const float* v_scale, const gqa_q8_kv_t* kv,
+                     const int32_t* block_table, const int32_t* seq_len, const int32_t* cu_new, int32_t batch,
+                     int32_t n_tokens, int32_t max_new, uint16_t* out, void* workspace, size_t workspace_bytes,
+                     void* stream) {
+    if (!params || !kv) return GQA_ERR_BAD_POINTER;
+    if (!geometry_ok(params) || (params->flags & GQA_ROPE_K) || !q8_layout_ok(kv) || kv->max_blocks <= 0 ||
+        kv->max_blocks > 0x7FFFFFF || batch <= 0 || batch > (1 << 27) || n_tokens <= 0 || max_new <= 0)
+        return GQA_ERR_INVALID_CONFIG;
+    if (!cu_new && n_tokens < batch) return GQA_ERR_INVALID_CONFIG;
+    if (q_token_stride < 0) return GQA_ERR_INVALID_CONFIG;
+    if (!q || !k_pool || !v_pool || !k_scale || !v_scale || !block_table || !seq_len || !out) return GQA_ERR_BAD_POINTER;
+    if (!aligned(q, 16) || q_token_stride % 8 || !aligned(out, 8) || !aligned(block_table, 4) || !aligned(seq_len, 4) ||
+        !aligned(cu_new, 4) || !q8_pool_aligned(kv, k_pool, v_pool, k_scale, v_scale))
+        return GQA_ERR_BAD_POINTER;
+    if (!workspace || !aligned(workspace, 256) ||
+        workspace_bytes < gqa_attention_q8_workspace_bytes(params, batch, n_tokens, max_new))
+        return GQA_ERR_WORKSPACE;
+    const int64_t rows = q8_rows(params, max_new);
+    Q8AttnArgs a{};
+    a.pool = q8_pool(kv, k_pool, v_pool, k_scale, v_scale);
+    a.q = q;
+    a.q_token_stride = q_token_stride;
+    a.block_table = block_table;
+    a.seq_len = seq_len;
+    a.cu = cu_new;
+    a.out = out;
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = reinterpret_cast<float4*>(static_cast<char*>(workspace) + align_up(static_cast<size_t>(rows) * kD * sizeof(float), 256));
+    a.tile_slot0 = q8_stream_rows(params, max_new);
+    a.max_blocks = kv->max_blocks;
+    a.batch = batch;
+    a.n_tokens = n_tokens;
+    a.max_new = max_new;
+    a.stream_waves = q8_stream_waves(params, max_new);
+    a.tile_wgs = q8_tile_wgs(params);
+    a.rope = (params->flags & GQA_ROPE_Q) != 0;
+    a.q_scale = static_cast<float>(qk_scale_log2(params));
+    if (a.rope) fill_rope_table(params->rope_theta, &a.rope_table);
+    return launch_q8_attention(a, kv->format, static_cast<hipStream_t>(stream)) == hipSuccess ? GQA_OK : GQA_ERR_HIP;
 }
 
 }  // extern "C"

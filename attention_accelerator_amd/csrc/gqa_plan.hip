@@ -1,0 +1,148 @@
+// gqa_plan.hip -- block tables and slot maps of a serving step, built on the GPU from the
+// requests' lengths.
+//
+// Request b has c cached positions and n new tokens; it takes need = ceil((c + n) / 16) -
+// ceil(c / 16) ids from the top of the stack of free blocks, first come, first served: granted
+// where the needs up to and with its own fit.  Two running sums over the requests therefore
+// decide everything: cu (token rows) and C (blocks).
+//
+// One launch and no traffic between workgroups: each workgroup owns a stretch of token rows and
+// forms the running sums itself, 1024 requests at a time with a carry, keeping the stretch of
+// them that its rows fall in; a row finds its request by bisection in LDS.  An id that a row
+// needs comes from the stack directly (never from a table entry that another workgroup
+// writes), and the row that opens a block writes the table's entry.  The arithmetic is tiny: a
+// call is bound by its launch and three dependent memory round trips (lengths, count of free
+// blocks and ids).
+#include "gqa_device.h"
+#include "gqa_internal.h"
+#include "gqa_q8.h"
+
+namespace gqa {
+
+namespace {
+
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanWaves = kPlanThreads / kWave;
+constexpr int32_t kMaxSlotBlock = 1 << 27;         // ids whose slots are int32
+
+template <typename T>
+__device__ __forceinline__ T wave_incl_scan(T x, int lane) {
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+        const T y = __shfl_up(x, d);
+        if (lane >= d) x += y;
+    }
+    return x;
+}
+
+// Inclusive sum over the workgroup's threads; `total`: of all of them.  `part`: LDS.
+template <typename T>
+__device__ __forceinline__ T block_incl_scan(T x, T* part, T& total) {
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
+    x = wave_incl_scan(x, lane);
+    if (lane == kWave - 1) part[wave] = x;
+    __syncthreads();
+    T before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < kPlanWaves; ++w) {
+        before += w < wave ? part[w] : T{0};
+        all += part[w];
+    }
+    __syncthreads();
+    total = all;
+    return x + before;
+}
+
+}  // namespace
+
+__global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs a) {
+    __shared__ int32_t s_cu[kPlanThreads];          // first row of each request of the window
+    __shared__ int32_t s_cached[kPlanThreads];      // positions it holds, -1: refused
+    __shared__ int32_t s_first[kPlanThreads];       // stack index of its first new block
+    __shared__ int64_t s_part64[kPlanWaves];
+    __shared__ int32_t s_part32[kPlanWaves];
+    const int tid = threadIdx.x;
+    const int64_t row0 = static_cast<int64_t>(blockIdx.x) * a.rows_per_wg;
+    const int64_t row1 = min(row0 + a.rows_per_wg, static_cast<int64_t>(a.n_rows));
+    const int32_t n_free = max(0, min(*a.n_free, a.free_capacity));
+    const int64_t capacity = static_cast<int64_t>(a.max_blocks) * kQ8Block;
+    int64_t rows_before = 0;                        // rows and blocks of the windows before
+    int32_t blocks_before = 0, blocks_used = 0;
+    for (int32_t b0 = 0, window = 0; b0 < a.batch; b0 += kPlanThreads, ++window) {
+        const int32_t b = b0 + tid;
+        int32_t c = 0, n = 0;
+        if (b < a.batch) {
+            c = a.cached[b];
+            n = a.n_new[b];
+        }
+        int64_t rows = 0;
+        const int64_t upto = rows_before + block_incl_scan<int64_t>(max(n, 0), s_part64, rows);
+        const bool valid = b < a.batch && n >= 0 && c >= 0 && static_cast<int64_t>(c) + n <= capacity && upto <= a.n_rows;
+        const int32_t had = (c >> 4) + ((c & 15) != 0);
+        const int32_t need = valid ? static_cast<int32_t>((static_cast<int64_t>(c) + n + 15) >> 4) - had : 0;
+        int32_t blocks = 0;
+        const int32_t taken = blocks_before + block_incl_scan<int32_t>(need, s_part32, blocks);
+        const bool granted = valid && (need == 0 || taken <= n_free);
+        const int64_t first_row = upto - max(n, 0);
+        s_cu[tid] = static_cast<int32_t>(min(first_row, static_cast<int64_t>(INT32_MAX)));
+        s_cached[tid] = granted ? c : -1;
+        s_first[tid] = n_free - 1 - (taken - need);
+        // The most blocks that fit: the running sum never falls, so it is the largest that does.
+        const int32_t fits = taken <= n_free ? taken : 0;
+        const uint64_t any = __ballot(taken <= n_free);
+        const int last = any ? 63 - __clzll(any) : 0;
+        const int32_t wave_fits = __shfl(fits, last);
+        if ((tid & (kWave - 1)) == 0) s_part32[tid >> 6] = wave_fits;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kPlanWaves; ++w) blocks_used = max(blocks_used, s_part32[w]);
+        // Each request's results, the windows dealt over the workgroups.
+        if (static_cast<uint32_t>(window) % gridDim.x == blockIdx.x && b < a.batch) {
+            a.cu_new[b] = s_cu[tid];
+            if (b == a.batch - 1) a.cu_new[a.batch] = static_cast<int32_t>(min(upto, static_cast<int64_t>(INT32_MAX)));
+            a.seq_len[b] = granted ? c + n : 0;
+        }
+        // The window's rows that are this workgroup's.
+        const int64_t lo = max(row0, rows_before), hi = min(row1, rows_before + rows);
+        const int32_t count = min(a.batch - b0, kPlanThreads);
+        for (int64_t t = lo + tid; t < hi; t += kPlanThreads) {
+            int at = 0;                             // the last request whose first row is <= t
+#pragma unroll
+            for (int step = kPlanThreads / 2; step; step >>= 1)
+                at += (at + step < count && s_cu[at + step] <= t) ? step : 0;
+            const int32_t held = s_cached[at];
+            int32_t slot = -1, pos = 0;
+            if (held >= 0) {
+                pos = held + static_cast<int32_t>(t - s_cu[at]);
+                const int32_t j = pos >> 4, own = (held >> 4) + ((held & 15) != 0);
+                int32_t* entry = a.block_table + static_cast<int64_t>(b0 + at) * a.table_stride + j;
+                const int32_t id = j < own ? *entry : a.free_blocks[s_first[at] - (j - own)];
+                if ((pos & 15) == 0) *entry = id;
+                slot = id >= 0 && id < kMaxSlotBlock ? id * kQ8Block + (pos & 15) : -1;
+            }
+            a.slot_map[t] = slot;
+            a.positions[t] = pos;
+        }
+        rows_before += rows;
+        blocks_before += blocks;
+        __syncthreads();
+    }
+    if (blockIdx.x == 0 && tid == 0) *a.n_free_out = n_free - blocks_used;
+    for (int64_t t = max(row0, rows_before) + tid; t < row1; t += kPlanThreads) {   // behind the last request
+        a.slot_map[t] = -1;
+        a.positions[t] = 0;
+    }
+}
+
+hipError_t launch_paged_plan(const PagedPlanArgs& args, hipStream_t stream) {
+    // A thousand rows for each workgroup, more where that would be over a thousand workgroups:
+    // each of them forms the running sums again.
+    PagedPlanArgs a = args;
+    const int64_t per = (static_cast<int64_t>(a.n_rows) + 1023) / 1024;
+    a.rows_per_wg = static_cast<int32_t>(per < kPlanThreads ? kPlanThreads : per);
+    const int64_t wgs = (static_cast<int64_t>(a.n_rows) + a.rows_per_wg - 1) / a.rows_per_wg;
+    hipLaunchKernelGGL(paged_plan_kernel, dim3(static_cast<unsigned>(wgs < 1 ? 1 : wgs)), dim3(kPlanThreads), 0, stream, a);
+    return hipGetLastError();
+}
+
+}  // namespace gqa

@@ -1,0 +1,123 @@
+// gqa_q8.h -- what the kernels of the 8-bit paged cache share: argument blocks, the two formats'
+// conversions, and one step of attention over 32 keys.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "gqa_device.h"
+
+namespace gqa {
+
+constexpr int kQ8Block = 16;               // positions of a block
+constexpr int kQ8Step = 32;                // keys of a step: two blocks
+constexpr int kQ8RowB = kD;                // a row's bytes
+constexpr int kQ8PlaneB = kQ8Step * kQ8RowB;   // K (or V) of a step in LDS
+constexpr int kQ8Int8 = 0;
+constexpr int kQ8E4m3 = 1;
+
+struct Q8Pool {
+    const uint8_t* k;
+    const uint8_t* v;
+    const float* k_scale;
+    const float* v_scale;
+    int64_t block_stride, head_stride, pos_stride;     // bytes
+    int64_t scale_block_stride, scale_head_stride;     // floats
+    int32_t n_blocks;
+};
+
+struct Q8AppendArgs {
+    Q8Pool pool;                           // (written through here: the entry point owns the cast)
+    const uint16_t* k_new;
+    const uint16_t* v_new;
+    int64_t k_token_stride, v_token_stride;            // elements
+    const int32_t* slots;
+    const int32_t* positions;
+    int32_t n_tokens;
+    int32_t rope;
+    RopeTable rope_table;
+};
+
+struct Q8AttnArgs {
+    Q8Pool pool;
+    const uint16_t* q;
+    int64_t q_token_stride;                // elements
+    const int32_t* block_table;
+    const int32_t* seq_len;
+    const int32_t* cu;                     // nullptr: one token for each sequence
+    uint16_t* out;
+    float* part_o;                         // partial O rows, 128 floats each
+    float4* part_ml;                       // (m, M, l, -) of each partial row
+    int64_t tile_slot0;                    // first partial row of the tile kernel's part
+    int32_t max_blocks;
+    int32_t batch;
+    int32_t n_tokens;
+    int32_t max_new;
+    int32_t stream_waves;                  // ranges of the stream kernel
+    int32_t tile_wgs;                      // workgroups of the tile kernel
+    int32_t rope;
+    float q_scale;                         // scale * log2(e)
+    RopeTable rope_table;
+};
+
+struct PagedPlanArgs {
+    const int32_t* cached;
+    const int32_t* n_new;
+    const int32_t* free_blocks;
+    const int32_t* n_free;
+    int32_t* block_table;
+    int64_t table_stride;
+    int32_t* seq_len;
+    int32_t* cu_new;
+    int32_t* slot_map;
+    int32_t* positions;
+    int32_t* n_free_out;
+    int32_t batch;
+    int32_t max_blocks;
+    int32_t free_capacity;
+    int32_t n_rows;
+    int32_t rows_per_wg;
+};
+
+hipError_t launch_paged_plan(const PagedPlanArgs& a, hipStream_t stream);
+hipError_t launch_q8_append(const Q8AppendArgs& a, int format, hipStream_t stream);
+hipError_t launch_q8_attention(const Q8AttnArgs& a, int format, hipStream_t stream);
+
+// A chunk of more than kQ8StreamMax tokens of one sequence goes to the tile kernel.
+constexpr int kQ8StreamMax = 16;
+constexpr int kQ8TileTokens = 64;
+
+constexpr int kQ8TileWgsPerCu = 1;
+
+// Ranges of the stream kernel for each CU: what its LDS and registers let run at once.
+constexpr int q8_waves_per_cu(int max_new) { return max_new <= 8 ? 8 : 4; }
+
+// Columns (token, head) of a stream workgroup in tiles of 16: 4 tokens x 4 heads each.
+__host__ __device__ constexpr int q8_stream_tiles(int max_new) { return max_new <= 4 ? 1 : max_new <= 8 ? 2 : 4; }
+
+typedef _Float16 q8_f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 q8_f16x8 __attribute__((ext_vector_type(8)));
+typedef int q8_i32x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) void q8_lds_void;
+typedef __attribute__((address_space(3))) q8_i32x2 q8_lds_i32x2;
+
+// Two codes of w (bytes 0-1 or 2-3) as fp16: exact for both formats.  int8: the byte with its
+// sign bit flipped is the low byte of the fp16 number 1024 + (code + 128).
+template <int kFmt, bool kHigh>
+__device__ __forceinline__ q8_f16x2 q8_pair(uint32_t w) {
+    if constexpr (kFmt == kQ8E4m3) {
+        return __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, kHigh);
+    } else {
+        const uint32_t p = __builtin_amdgcn_perm(0x64646464u, w ^ 0x80808080u, kHigh ? 0x04030402u : 0x04010400u);
+        return __builtin_bit_cast(q8_f16x2, p) - q8_f16x2{(_Float16)1152.0f, (_Float16)1152.0f};
+    }
+}
+
+template <int kFmt>
+__device__ __forceinline__ q8_f16x8 q8_eight(uint32_t w0, uint32_t w1) {
+    const q8_f16x2 a = q8_pair<kFmt, false>(w0), b = q8_pair<kFmt, true>(w0);
+    const q8_f16x2 c = q8_pair<kFmt, false>(w1), d = q8_pair<kFmt, true>(w1);
+    return q8_f16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+
+}  // namespace gqa

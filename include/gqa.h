@@ -262,6 +262,93 @@ int gqa_kv_append_bf16(const gqa_params_t* params, const uint16_t* k_new, const 
                        uint16_t* k_cache, uint16_t* v_cache, const gqa_kv_layout_t* kv,
                        const int32_t* start, int32_t batch, int32_t n_new, void* stream);
 
+/* Block tables and slot maps of a serving step, from the requests' lengths (no counterpart in
+ * the reference, which has one sequence).  Request b holds cached[b] positions and brings
+ * n_new[b] tokens; block ids are taken from the top of a stack of free ones:
+ *   cached, n_new  [batch] int32
+ *   free_blocks    [free_capacity] int32, the stack; *n_free of them are free (read as at most
+ *                  free_capacity, at least 0)
+ *   block_table    int32, row b at b * table_stride, max_blocks entries; entries of new blocks
+ *                  are written, the others kept
+ *   seq_len        [batch]: cached + n_new, or 0 for a refused request
+ *   cu_new         [batch + 1]: first token row of each request (a negative n_new has none), and
+ *                  the end
+ *   slot_map, positions [n_rows]: token i of request b (row cu_new[b] + i) is position cached[b] +
+ *                  i, slot 16 * id of its block + position % 16; -1 and 0 for a refused
+ *                  request's rows and the rows behind the last request
+ *   n_free_out     [1]: what is left of the stack
+ * A request takes ceil((cached + n_new) / 16) - ceil(cached / 16) blocks, first come, first
+ * served: it is granted where the needs of the requests up to it fit (and always where it
+ * needs none), else refused whole: its entries, slots and length as above.  Refused too:
+ * negative values, more than 16 * max_blocks positions, rows past n_rows (these count for no
+ * other request).  All arrays are device memory, and no output may overlap an input (the
+ * block table's kept entries are read; n_free_out is not n_free).  n_new[b] == 0 is a request at
+ * rest. */
+int gqa_paged_plan(const int32_t* cached, const int32_t* n_new, int32_t batch, const int32_t* free_blocks,
+                   const int32_t* n_free, int32_t free_capacity, int32_t* block_table, int64_t table_stride,
+                   int32_t max_blocks, int32_t n_rows, int32_t* seq_len, int32_t* cu_new, int32_t* slot_map,
+                   int32_t* positions, int32_t* n_free_out, void* stream);
+
+/* 8-bit paged cache: pools as gqa_paged_kv_t's, of one byte an element, with a float scale for
+ * each (block, KV head) of K and of V: an element stands for code * scale.  Formats: int8
+ * (-127 .. 127) and OCP e4m3 (448 at most).  Row (block id, KV head h, position r) starts at byte
+ * id*block_stride + h*head_stride + r*pos_stride (128 bytes; strides multiples of 16, pools
+ * 16-byte aligned, 16 * pos_stride below 2^31), its scale is element id*scale_block_stride +
+ * h*scale_head_stride.  A scale is a finite number, not negative; powers of two where
+ * gqa_kv_append_q8 wrote it. */
+#define GQA_Q8_INT8 0
+#define GQA_Q8_E4M3 1
+typedef struct gqa_q8_kv {
+    int64_t block_stride;         /* bytes */
+    int64_t head_stride;
+    int64_t pos_stride;
+    int64_t scale_block_stride;   /* floats */
+    int64_t scale_head_stride;
+    int32_t block_size;           /* must be 16 */
+    int32_t max_blocks;           /* block-table entries per sequence (attention) */
+    int32_t n_blocks;             /* blocks in the pool, at most 2^27 - 1 */
+    int32_t format;               /* GQA_Q8_INT8 or GQA_Q8_E4M3 */
+} gqa_q8_kv_t;
+
+/* KV append into an 8-bit pool, ragged: token t (row h of it at t*token_stride + 128 h elements,
+ * strides multiples of 4, pointers 8-byte aligned) goes to slot slots[t] = 16 * block + row; a slot
+ * outside the pool (-1) is skipped.  K is rotated at positions[t] when GQA_ROPE_K and rounded
+ * double -> f32, V is taken as it is.  The rows that a call puts into one block share its scale
+ * per KV head: the smallest power of two s with s * qmax (127, 448) at least their largest finite
+ * magnitude, and at least 2^-126; where the first of them is not row 0, at least the block's
+ * present scale, and where it grows the rows before it are requantised (code * old / new).  Codes
+ * are rounded to nearest even and saturate; a NaN becomes e4m3's NaN, 0 in int8.  A present scale
+ * that is not a positive finite number counts as 0.  The tokens of one block have to follow each
+ * other in the call (skipped ones aside), each slot at most once, and no two sequences may write one block: a block is
+ * read, scaled and written by one workgroup.  positions may be NULL without GQA_ROPE_K. */
+int gqa_kv_append_q8(const gqa_params_t* params, const uint16_t* k_new, int64_t k_token_stride,
+                     const uint16_t* v_new, int64_t v_token_stride, void* k_pool, void* v_pool, float* k_scale,
+                     float* v_scale, const gqa_q8_kv_t* kv, const int32_t* slots, const int32_t* positions,
+                     int32_t n_tokens, void* stream);
+
+/* Ragged attention over an 8-bit paged cache: sequence b has the query rows cu_new[b] ..
+ * cu_new[b+1] - 1 (cu_new [batch + 1], NULL: row b alone), the last of its seq_len[b] positions, all
+ * of them in the cache: row t of its n attends to keys p <= seq_len[b] - n + t, rotated at that
+ * position when GQA_ROPE_Q; the cache holds post-RoPE K (GQA_ROPE_K is rejected).
+ *   q      row r, head i at r*q_token_stride + 128 i elements (stride a multiple of 8, 16-byte
+ *          aligned); n_tokens rows
+ *   out    [n_tokens][32][128]; rows that belong to no sequence are left as they were
+ *   max_new  at least every sequence's rows (a host bound; it chooses the kernels)
+ *   workspace  gqa_attention_q8_workspace_bytes bytes, 256-byte aligned, any contents
+ * A sequence of up to 16 rows is streamed: the keys of all (sequence, KV head) pairs are cut into
+ * equal ranges; longer ones go in tiles of 64 rows.  A sequence with seq_len[b] below its rows or
+ * above 16 * max_blocks, or more than max_new rows, gets NaN rows; where cu_new is not
+ * ascending within [0, n_tokens] nothing is written for the sequence.  Rows that attend to a block
+ * whose id is outside [0, n_blocks), or whose scale is negative or NaN, are NaN.  What the cache
+ * holds behind seq_len[b], or in keys a row does not see, does not reach it.  Arithmetic: fp16
+ * products of exact codes with Q and weights of 11 bits, fp32 sums, one BF16 rounding. */
+size_t gqa_attention_q8_workspace_bytes(const gqa_params_t* params, int32_t batch, int32_t n_tokens, int32_t max_new);
+int gqa_attention_q8(const gqa_params_t* params, const uint16_t* q, int64_t q_token_stride, const void* k_pool,
+                     const void* v_pool, const float* k_scale, const float* v_scale, const gqa_q8_kv_t* kv,
+                     const int32_t* block_table, const int32_t* seq_len, const int32_t* cu_new, int32_t batch,
+                     int32_t n_tokens, int32_t max_new, uint16_t* out, void* workspace, size_t workspace_bytes,
+                     void* stream);
+
 /* rope_unit in isolation (rope_unit.v:38-330 as tests/tb_rope_unit.sv drives it;
  * golden pyfiles/gen_rope_test_vectors.py:16-20): out[r] = BF16(rope(in[r], position)),
  * position = positions[r] if positions != NULL (device int32) else pos0 + r.
@@ -294,8 +381,9 @@ int gqa_profile_read_stages(double* stage_ms, int32_t n_stages, int32_t* calls);
 const char* gqa_status_string(int status);
 
 /* ABI version: (major << 16) | minor.  It tells callers what of the declarations above they may
- * rely on, but for gqa_decode_host_bf16 and gqa_decode_host_workspace_bytes: they came after 4.1
- * without a new minor number, so a caller that may meet an older library looks the symbol up. */
+ * rely on, but for gqa_decode_host_bf16, gqa_decode_host_workspace_bytes, gqa_paged_plan and the _q8
+ * functions: they came after 4.1 without a new minor number, so a caller that may meet an older
+ * library looks the symbol up. */
 uint32_t gqa_abi_version(void);
 
 #ifdef __cplusplus
