@@ -21,7 +21,7 @@ from .attention import (DEFAULT_SCALE, GROUP_SIZE, HEAD_DIM, N_KV_HEADS, N_Q_HEA
                         profile_enable, profile_read, profile_read_stages, rope_half_split,
                         validate_lengths)
 from .paged_q8 import (PagedPlan, PreparedAttentionQ8, Q8Pool, attention_q8_workspace_bytes,  # noqa: F401
-                       gqa_attention_q8, kv_append_q8, new_q8_pool, paged_plan)
+                       gqa_attention_q8, kv_append_q8, new_attention_q8_workspace, new_q8_pool, paged_plan)
 from ._lib import GqaConfigError, GqaError  # noqa: F401
 
 __version__ = "0.1.0"

@@ -50,6 +50,7 @@ EXPORTS = (
     "gqa_paged_plan",
     "gqa_kv_append_q8",
     "gqa_attention_q8_workspace_bytes",
+    "gqa_attention_q8_workspace_init",
     "gqa_attention_q8",
     "gqa_rope_rows_bf16",
     "gqa_profile_enable",
@@ -191,6 +192,8 @@ def lib() -> ctypes.CDLL:
     L.gqa_kv_append_q8.restype = ctypes.c_int
     L.gqa_attention_q8_workspace_bytes.argtypes = [ctypes.POINTER(GqaParams), i32, i32, i32]
     L.gqa_attention_q8_workspace_bytes.restype = ctypes.c_size_t
+    L.gqa_attention_q8_workspace_init.argtypes = [vp, ctypes.c_size_t, vp]
+    L.gqa_attention_q8_workspace_init.restype = ctypes.c_int
     L.gqa_attention_q8.argtypes = [ctypes.POINTER(GqaParams), vp, i64, vp, vp, vp, vp, ctypes.POINTER(GqaQ8Kv),
                                    vp, vp, vp, i32, i32, i32, vp, vp, ctypes.c_size_t, vp]
     L.gqa_attention_q8.restype = ctypes.c_int

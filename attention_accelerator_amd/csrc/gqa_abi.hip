@@ -783,10 +783,10 @@ Q8Pool q8_pool(const gqa_q8_kv_t* kv, const void* k, const void* v, const float*
     return p;
 }
 
-// Ranges of the stream kernel (one-wave workgroups) and workgroups of the tile kernel.
-int32_t q8_stream_waves(const gqa_params_t* p, int32_t max_new) {
-    const int32_t cus = stream_wgs(p) / kWavesPerCu;
-    return cus > 0 ? cus * q8_waves_per_cu(max_new) : 1;
+// One-wave workgroups of the stream kernel (a range for every eight of them) and workgroups of the tile kernel.
+int32_t q8_stream_waves(const gqa_params_t* p) {
+    const int32_t waves = stream_wgs(p) / kWavesPerCu * kQ8WavesPerCu / kHkv * kHkv;
+    return waves > 0 ? waves : kHkv;
 }
 
 int32_t q8_tile_wgs(const gqa_params_t* p) {
@@ -794,9 +794,13 @@ int32_t q8_tile_wgs(const gqa_params_t* p) {
     return cus > 0 ? cus * kQ8TileWgsPerCu : 1;
 }
 
+// A workspace begins with the stream kernel's counters, at the same place and of the same size for every
+// call: what one call's partials lie in is never another's counters.
+constexpr size_t kQ8CounterBytes = size_t{kQ8MaxBatch} * kHkv * sizeof(uint32_t);
+
 // Partial rows of the stream kernel (two pieces of every range), then of the tile kernel.
 int64_t q8_stream_rows(const gqa_params_t* p, int32_t max_new) {
-    return int64_t{2} * q8_stream_waves(p, max_new) * 16 * q8_stream_tiles(max_new);
+    return int64_t{2} * q8_stream_waves(p) * (max_new == 1 ? kGroup : 16 * q8_stream_tiles(max_new));
 }
 
 int64_t q8_rows(const gqa_params_t* p, int32_t max_new) {
@@ -876,9 +880,16 @@ int gqa_kv_append_q8(const gqa_params_t* params, const uint16_t* k_new, int64_t 
 }
 
 size_t gqa_attention_q8_workspace_bytes(const gqa_params_t* params, int32_t batch, int32_t n_tokens, int32_t max_new) {
-    if (!params || !geometry_ok(params) || batch <= 0 || n_tokens <= 0 || max_new <= 0) return 0;
+    if (!params || !geometry_ok(params) || batch <= 0 || batch > kQ8MaxBatch || n_tokens <= 0 || max_new <= 0) return 0;
     const size_t rows = static_cast<size_t>(q8_rows(params, max_new));
-    return align_up(rows * kD * sizeof(float), 256) + align_up(rows * sizeof(float4), 256);
+    return kQ8CounterBytes + align_up(rows * kD * sizeof(float), 256) + align_up(rows * sizeof(float4), 256);
+}
+
+int gqa_attention_q8_workspace_init(void* workspace, size_t workspace_bytes, void* stream) {
+    if (!workspace || workspace_bytes < kQ8CounterBytes || !aligned(workspace, 256)) return GQA_ERR_WORKSPACE;
+    const hipError_t e = launch_zero_words(static_cast<uint32_t*>(workspace), static_cast<int64_t>(kQ8CounterBytes / 4),
+                                           static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? GQA_OK : GQA_ERR_HIP;
 }
 
 int gqa_attention_q8(const gqa_params_t* params, const uint16_t* q, int64_t q_token_stride, const void* k_pool,
@@ -888,7 +899,7 @@ int gqa_attention_q8(const gqa_params_t* params, const uint16_t* q, int64_t q_to
                      void* stream) {
     if (!params || !kv) return GQA_ERR_BAD_POINTER;
     if (!geometry_ok(params) || (params->flags & GQA_ROPE_K) || !q8_layout_ok(kv) || kv->max_blocks <= 0 ||
-        kv->max_blocks > 0x7FFFFFF || batch <= 0 || batch > (1 << 27) || n_tokens <= 0 || max_new <= 0)
+        kv->max_blocks >= (1 << 26) || batch <= 0 || batch > kQ8MaxBatch || n_tokens <= 0 || max_new <= 0)
         return GQA_ERR_INVALID_CONFIG;
     if (!cu_new && n_tokens < batch) return GQA_ERR_INVALID_CONFIG;
     if (q_token_stride < 0) return GQA_ERR_INVALID_CONFIG;
@@ -908,14 +919,16 @@ int gqa_attention_q8(const gqa_params_t* params, const uint16_t* q, int64_t q_to
     a.seq_len = seq_len;
     a.cu = cu_new;
     a.out = out;
-    a.part_o = static_cast<float*>(workspace);
-    a.part_ml = reinterpret_cast<float4*>(static_cast<char*>(workspace) + align_up(static_cast<size_t>(rows) * kD * sizeof(float), 256));
+    a.counters = static_cast<uint32_t*>(workspace);
+    char* partials = static_cast<char*>(workspace) + kQ8CounterBytes;
+    a.part_o = reinterpret_cast<float*>(partials);
+    a.part_ml = reinterpret_cast<float4*>(partials + align_up(static_cast<size_t>(rows) * kD * sizeof(float), 256));
     a.tile_slot0 = q8_stream_rows(params, max_new);
     a.max_blocks = kv->max_blocks;
     a.batch = batch;
     a.n_tokens = n_tokens;
     a.max_new = max_new;
-    a.stream_waves = q8_stream_waves(params, max_new);
+    a.stream_waves = q8_stream_waves(params);
     a.tile_wgs = q8_tile_wgs(params);
     a.rope = (params->flags & GQA_ROPE_Q) != 0;
     a.q_scale = static_cast<float>(qk_scale_log2(params));

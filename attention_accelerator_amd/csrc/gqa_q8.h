@@ -46,6 +46,8 @@ struct Q8AttnArgs {
     const int32_t* seq_len;
     const int32_t* cu;                     // nullptr: one token for each sequence
     uint16_t* out;
+    uint32_t* counters;                    // [8][kQ8MaxBatch] pieces written (the heads' far apart: counts in one
+                                           // cache line wait for each other); 0 between calls
     float* part_o;                         // partial O rows, 128 floats each
     float4* part_ml;                       // (m, M, l, -) of each partial row
     int64_t tile_slot0;                    // first partial row of the tile kernel's part
@@ -53,7 +55,7 @@ struct Q8AttnArgs {
     int32_t batch;
     int32_t n_tokens;
     int32_t max_new;
-    int32_t stream_waves;                  // ranges of the stream kernel
+    int32_t stream_waves;                  // of the stream kernel: a multiple of 8
     int32_t tile_wgs;                      // workgroups of the tile kernel
     int32_t rope;
     float q_scale;                         // scale * log2(e)
@@ -83,14 +85,18 @@ hipError_t launch_paged_plan(const PagedPlanArgs& a, hipStream_t stream);
 hipError_t launch_q8_append(const Q8AppendArgs& a, int format, hipStream_t stream);
 hipError_t launch_q8_attention(const Q8AttnArgs& a, int format, hipStream_t stream);
 
+constexpr int32_t kQ8MaxBatch = 32768;     // sequences that the counters at a workspace's start are for
+
 // A chunk of more than kQ8StreamMax tokens of one sequence goes to the tile kernel.
 constexpr int kQ8StreamMax = 16;
 constexpr int kQ8TileTokens = 64;
 
 constexpr int kQ8TileWgsPerCu = 1;
 
-// Ranges of the stream kernel for each CU: what its LDS and registers let run at once.
-constexpr int q8_waves_per_cu(int max_new) { return max_new <= 8 ? 8 : 4; }
+// Waves of the stream kernel for each CU: one per SIMD.  (More of them read slower: HBM serves fewer
+// streams at once faster.)  Steps of a wave's ring in LDS (8 KB each).
+constexpr int kQ8WavesPerCu = 4;
+__host__ __device__ constexpr int q8_ring(int) { return 3; }
 
 // Columns (token, head) of a stream workgroup in tiles of 16: 4 tokens x 4 heads each.
 __host__ __device__ constexpr int q8_stream_tiles(int max_new) { return max_new <= 4 ? 1 : max_new <= 8 ? 2 : 4; }
@@ -98,8 +104,10 @@ __host__ __device__ constexpr int q8_stream_tiles(int max_new) { return max_new 
 typedef _Float16 q8_f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 q8_f16x8 __attribute__((ext_vector_type(8)));
 typedef int q8_i32x2 __attribute__((ext_vector_type(2)));
-typedef __attribute__((address_space(3))) void q8_lds_void;
-typedef __attribute__((address_space(3))) q8_i32x2 q8_lds_i32x2;
+typedef uint32_t q8_u32x4 __attribute__((ext_vector_type(4)));
+// LDS pointers keep their address space (32 bits, no generic-pointer checks).
+#define GQA_LDS __attribute__((address_space(3)))
+typedef GQA_LDS uint8_t q8_lds;
 
 // Two codes of w (bytes 0-1 or 2-3) as fp16: exact for both formats.  int8: the byte with its
 // sign bit flipped is the low byte of the fp16 number 1024 + (code + 128).
@@ -118,6 +126,12 @@ __device__ __forceinline__ q8_f16x8 q8_eight(uint32_t w0, uint32_t w1) {
     const q8_f16x2 a = q8_pair<kFmt, false>(w0), b = q8_pair<kFmt, true>(w0);
     const q8_f16x2 c = q8_pair<kFmt, false>(w1), d = q8_pair<kFmt, true>(w1);
     return q8_f16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+
+// Values as two fp16, to nearest (v_cvt_pk_f16_f32).
+__device__ __forceinline__ q8_f16x2 q8_pack(float lo, float hi) {
+    typedef float f32x2_t __attribute__((ext_vector_type(2)));
+    return __builtin_convertvector(f32x2_t{lo, hi}, q8_f16x2);
 }
 
 }  // namespace gqa

@@ -14,11 +14,15 @@
 //    pair of one KV head: col = 4 token + head.  The rows of the two key tiles are chosen so that
 //    lane (g, n) ends with the scores of keys 8g .. 8g+7 of column n: all of one block, so a
 //    lane has one sk and one sv, and its eight weights are its B operand of O^T = V^T P^T.
-//  * Two running maxima in fp32: m of the scores and M of s + log2(sv).  A weight is formed as
-//    w = 2^(s + log2 sv - M) <= 1 and rounded to fp16 for the products with V's codes: V's scale
-//    is inside the weight, and what fp16 loses is relative to the largest w of the column, not
-//    to that of a block of a larger scale.  The softmax sum takes 2^(s - m) = w 2^(M - log2 sv - m),
-//    one product for a lane's eight weights.  O = acc 2^(M - m) / l.
+//  * Two running references in fp32: m for the scores and M for s + log2(sv).  A weight is formed as
+//    w = 2^(s + log2 sv - M) and rounded to fp16 for the products with V's codes: V's scale is
+//    inside the weight, and what fp16 loses is relative to the largest w of the column, not to
+//    that of a block of a larger scale.  The softmax sum takes 2^(s - m) = w 2^(M - log2 sv - m), one
+//    product for the fp32 sum of a lane's eight weights (not the rounded ones: where a block's
+//    V scale is small, they hold few bits of s).  O = acc 2^(M - m) / l.
+//  * m and M are the maxima as of the last time a key lay more than 2^kSlack above one of them: up to
+//    there a weight is at most 2^kSlack, far inside fp16, and nothing has to be rescaled or even
+//    compared across lanes.
 //  * Keys that a column does not see get w = 0; V rows behind the sequence's end are cleared
 //    (they may hold anything, NaN codes too).
 #include "gqa_device.h"
@@ -29,7 +33,8 @@ namespace gqa {
 
 namespace {
 
-constexpr float kLowest = -3.0e38f;        // a running max before any key (finite: no inf - inf)
+constexpr float kLowest = -3.0e38f;        // a reference before any key (finite: no inf - inf)
+constexpr float kSlack = 8.0f;             // how far (log2) a key may lie above its reference
 
 // Tokens and first position of sequence b; false where it has no row to compute (lengths that
 // break the rules are the merge kernel's: NaN rows).
@@ -76,19 +81,27 @@ __device__ __forceinline__ int v_swizzle(int r) { return r & 7; }
 // Lane l's part of copy q (rows 8q .. 8q+7) of a step's plane.
 __device__ __forceinline__ int copy_row(int q, int lane) { return 8 * q + (lane >> 3); }
 
-// Q operands: B = Q^T of tile c, slice s: lane (g, n) holds column n's dims that lane (g, r)
-// holds of a key row: 16 (g + 4 (s / 2)) + 8 (s % 2) + j.  `cs`: (cos, sin) of the tile's tokens
-// [token][64] in LDS.  Returns the power of two the row was divided by.
-__device__ __forceinline__ float load_q(const Q8AttnArgs& a, const uint16_t* row, const float2* cs, int g,
-                                        q8_f16x8 (&op)[4]) {
-    float x[16], y[16];
+// This lane's part of a query row: dims 16 g .. 16 g + 15 and 64 on, what its B operands hold.
+struct Q8Row {
+    uint4 lo[2], hi[2];
+};
+
+__device__ __forceinline__ Q8Row fetch_q(const uint16_t* row, int g) {
     const uint4* lo = reinterpret_cast<const uint4*>(row + 16 * g);
     const uint4* hi = reinterpret_cast<const uint4*>(row + kPairs + 16 * g);
+    return Q8Row{{lo[0], lo[1]}, {hi[0], hi[1]}};
+}
+
+// Q operands: B = Q^T of a tile, slice s: lane (g, n) holds column n's dims that lane (g, r) holds of
+// a key row: 16 (g + 4 (s / 2)) + 8 (s % 2) + j.  `cs`: (cos, sin) of the column's token in LDS.
+// Returns the power of two the row was divided by.
+__device__ __forceinline__ float make_q(const Q8AttnArgs& a, const Q8Row& raw, const float2* cs, int g, q8_f16x8 (&op)[4]) {
+    float x[16], y[16];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         float f[8], e[8];
-        unpack8(lo[i], f);
-        unpack8(hi[i], e);
+        unpack8(raw.lo[i], f);
+        unpack8(raw.hi[i], e);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             x[8 * i + j] = f[j];
@@ -122,6 +135,10 @@ __device__ __forceinline__ float load_q(const Q8AttnArgs& a, const uint16_t* row
     return __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
 }
 
+__device__ __forceinline__ const uint16_t* q_row(const Q8AttnArgs& a, int row, int h, int head) {
+    return a.q + static_cast<int64_t>(row) * a.q_token_stride + (kGroup * h + head) * kD;
+}
+
 // cos and sin of `tokens` positions from `start` on, by `threads` threads (a token's 64 pairs by
 // 64 of them).
 __device__ __forceinline__ void fill_angles(const Q8AttnArgs& a, int start, int tokens, float2* cs, int tid, int threads) {
@@ -134,19 +151,25 @@ __device__ __forceinline__ void fill_angles(const Q8AttnArgs& a, int start, int 
     }
 }
 
-// 16 bytes per lane straight into LDS (lane l's at dst + 16 l): global_load_lds_dwordx4.  Inline, so
-// that the compiler does not make every later LDS read wait for all copies in flight; the
+// 16 (or 4) bytes per lane straight into LDS, lane l's at dst + 16 l (4 l): global_load_lds_*.  Inline,
+// so that the compiler does not make every later LDS read wait for all copies in flight; the
 // waits are explicit (wait_copies).
-__device__ __forceinline__ void copy16(const uint8_t* base, uint32_t off, const uint8_t* dst, bool stream) {
-    const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(q8_lds_void*)dst);
-    if (stream)
+template <bool kStream>
+__device__ __forceinline__ void copy16(const uint8_t* base, uint32_t off, q8_lds* dst) {
+    const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)dst);
+    if constexpr (kStream)
         asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(off), "s"(base), "{m0}"(at) : "memory");
     else
         asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(at) : "memory");
 }
 
+__device__ __forceinline__ void copy4(const void* src, q8_lds* dst) {
+    const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)dst);
+    asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "{m0}"(at) : "memory");
+}
+
 // Until at most kLeft of this wave's memory operations (copies, and any the compiler issued since)
-// are in flight.
+// are in flight: they end in the order they were issued in.
 template <int kLeft>
 __device__ __forceinline__ void wait_copies() {
     static_assert(kLeft <= 63, "vmcnt range");
@@ -159,30 +182,45 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
     return ~((x + 0x7f7f7f7fu) | x) & 0x80808080u;
 }
 
+// This lane's reads of a step's planes.  K: row 8 (r / 4) + r % 4 (tile 1: 4 rows on), chunks g and
+// g + 4.  V, transposed reads: of each 16 lanes, lane r names 8 bytes of row 8g + r / 2 and gets
+// dim r of the 8 rows.
+__device__ __forceinline__ uint32_t k_offset(int lane) {
+    const int g = lane >> 4, r = lane & 15, row = 8 * (r >> 2) + (r & 3);
+    return static_cast<uint32_t>(row * kQ8RowB + 16 * (g ^ k_swizzle(row)));
+}
+
+__device__ __forceinline__ uint32_t v_offset(int lane) {
+    const int g = lane >> 4, r = lane & 15, row = 8 * g + (r >> 1);
+    return static_cast<uint32_t>(row * kQ8RowB + 8 * (r & 1) + 16 * v_swizzle(row));
+}
+
+__device__ __forceinline__ q8_i32x2 read_v(const q8_lds* vp, uint32_t voff, int dt) {
+    return __builtin_amdgcn_ds_read_tr8_b64_v2i32((GQA_LDS q8_i32x2*)(vp + (voff ^ (16u * dt))));
+}
+
 // V of a step that some column does not see whole: rows behind `last` are cleared (they may hold
 // anything), and NaN codes, of which 0 * NaN would reach the columns that do not see their key,
 // are cleared too, after the elements of the columns that do see them have been marked.  Called by
 // all `threads` threads of the workgroup.
 template <int kFmt, int kTiles>
-__device__ __forceinline__ void mask_values(uint8_t* vp, int key0, int last, const int (&lim)[kTiles], int tid, int threads,
+__device__ __forceinline__ void mask_values(q8_lds* vp, int key0, int last, const int (&lim)[kTiles], int tid, int threads,
                                             Q8State<kTiles>& st) {
-    const int lane = tid & (kWave - 1), g = lane >> 4, r = lane & 15;
-    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+    const int lane = tid & (kWave - 1), g = lane >> 4;
     for (int row = tid >> 3; row < kQ8Step; row += threads >> 3)
-        if (key0 + row > last) *reinterpret_cast<uint4*>(vp + row * kQ8RowB + 16 * (tid & 7)) = zero;
+        if (key0 + row > last) *(GQA_LDS q8_u32x4*)(vp + row * kQ8RowB + 16 * (tid & 7)) = q8_u32x4{0u, 0u, 0u, 0u};
     __syncthreads();
     if constexpr (kFmt == kQ8E4m3) {
         uint32_t any = 0;
         for (int row = lane >> 3; row < kQ8Step; row += kWave >> 3) {
-            const uint4 w = *reinterpret_cast<const uint4*>(vp + row * kQ8RowB + 16 * (lane & 7));
+            const q8_u32x4 w = *(GQA_LDS q8_u32x4*)(vp + row * kQ8RowB + 16 * (lane & 7));
             any |= nan_bytes(w.x) | nan_bytes(w.y) | nan_bytes(w.z) | nan_bytes(w.w);
         }
         if (!__any(any != 0)) return;              // (the same for every wave: each looked at the whole plane)
-        const int vrow = 8 * g + (r >> 1);
+        const uint32_t voff = v_offset(lane);
 #pragma unroll 1
         for (int dt = 0; dt < 8; ++dt) {
-            const q8_i32x2 v = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                (q8_lds_i32x2*)(vp + vrow * kQ8RowB + 8 * (r & 1) + 16 * (dt ^ v_swizzle(vrow))));
+            const q8_i32x2 v = read_v(vp, voff, dt);
             const uint64_t bits =
                 nan_bytes(static_cast<uint32_t>(v.x)) | (static_cast<uint64_t>(nan_bytes(static_cast<uint32_t>(v.y))) << 32);
             q8_f16x8 is;
@@ -201,36 +239,50 @@ __device__ __forceinline__ void mask_values(uint8_t* vp, int key0, int last, con
         }
         __syncthreads();
         for (int row = tid >> 3; row < kQ8Step; row += threads >> 3) {
-            uint4* at = reinterpret_cast<uint4*>(vp + row * kQ8RowB + 16 * (tid & 7));
-            uint4 w = *at;
-            w.x &= ~(nan_bytes(w.x) / 0x80u * 0xffu);
-            w.y &= ~(nan_bytes(w.y) / 0x80u * 0xffu);
-            w.z &= ~(nan_bytes(w.z) / 0x80u * 0xffu);
-            w.w &= ~(nan_bytes(w.w) / 0x80u * 0xffu);
+            GQA_LDS q8_u32x4* at = (GQA_LDS q8_u32x4*)(vp + row * kQ8RowB + 16 * (tid & 7));
+            q8_u32x4 w = *at;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] &= ~(nan_bytes(w[i]) / 0x80u * 0xffu);
             *at = w;
         }
         __syncthreads();
     }
 }
 
-// One step: 32 keys from position key0 on, in the LDS planes kp and vp.  sk, lsv: this lane's
-// block's K scale and log2 of its V scale; qs: the columns' powers of two; lim: the last
-// position each column sees; masked: some column does not see all 32 keys.
-template <int kFmt, int kTiles>
-__device__ __forceinline__ void q8_step(const uint8_t* kp, const uint8_t* vp, int key0, bool masked, float sk, float lsv,
-                                        const q8_f16x8 (&qop)[kTiles][4], const float (&qs)[kTiles],
-                                        const int (&lim)[kTiles], int lane, Q8State<kTiles>& st) {
-    const int g = lane >> 4, r = lane & 15;
-    f32x4_t s[kTiles][2];
+// A step's operands as they lie in LDS.  They are read all at once, ahead of their use: left to itself
+// the compiler reads each one just before its product and waits for it.
+struct Q8KRows {
+    q8_u32x4 w[2][2];                      // [tile][chunk g, g + 4]
+};
+
+struct Q8VRows {
+    q8_i32x2 w[8];                         // [16 dims]
+};
+
+__device__ __forceinline__ Q8KRows read_keys(const q8_lds* kp, uint32_t koff) {
+    Q8KRows k;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-        const int row = 8 * (r >> 2) + (r & 3) + 4 * t;
-        const uint8_t* p = kp + row * kQ8RowB;
-        const int at = g ^ k_swizzle(row);
-        const uint4 w0 = *reinterpret_cast<const uint4*>(p + 16 * at);
-        const uint4 w1 = *reinterpret_cast<const uint4*>(p + 16 * (at ^ 4));
-        const q8_f16x8 k0 = q8_eight<kFmt>(w0.x, w0.y), k1 = q8_eight<kFmt>(w0.z, w0.w);
-        const q8_f16x8 k2 = q8_eight<kFmt>(w1.x, w1.y), k3 = q8_eight<kFmt>(w1.z, w1.w);
+        k.w[t][0] = *(const GQA_LDS q8_u32x4*)(kp + koff + 4 * kQ8RowB * t);
+        k.w[t][1] = *(const GQA_LDS q8_u32x4*)(kp + (koff ^ 64u) + 4 * kQ8RowB * t);
+    }
+    return k;
+}
+
+__device__ __forceinline__ Q8VRows read_values(const q8_lds* vp, uint32_t voff) {
+    Q8VRows v;
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) v.w[dt] = read_v(vp, voff, dt);
+    return v;
+}
+
+// S^T of 32 keys: s[c][t][i] is the score of key 8g + 4t + i for column n of tile c.
+template <int kFmt, int kTiles>
+__device__ __forceinline__ void q8_scores(const Q8KRows& k, const q8_f16x8 (&qop)[kTiles][4], f32x4_t (&s)[kTiles][2]) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const q8_f16x8 k0 = q8_eight<kFmt>(k.w[t][0].x, k.w[t][0].y), k1 = q8_eight<kFmt>(k.w[t][0].z, k.w[t][0].w);
+        const q8_f16x8 k2 = q8_eight<kFmt>(k.w[t][1].x, k.w[t][1].y), k3 = q8_eight<kFmt>(k.w[t][1].z, k.w[t][1].w);
 #pragma unroll
         for (int c = 0; c < kTiles; ++c) {
             f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -240,104 +292,206 @@ __device__ __forceinline__ void q8_step(const uint8_t* kp, const uint8_t* vp, in
             s[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k3, qop[c][3], acc, 0, 0, 0);
         }
     }
-    // Weights: lane (g, n) has keys key0 + 8g + j.
-    q8_f16x8 p[kTiles];
+}
+
+__device__ __forceinline__ float max8(const f32x4_t (&s)[2]) {
+    const float a = fmaxf(fmaxf(s[0][0], s[0][1]), s[0][2]), b = fmaxf(fmaxf(s[0][3], s[1][0]), s[1][1]);
+    return fmaxf(fmaxf(a, b), fmaxf(s[1][2], s[1][3]));
+}
+
+// A step's scores made ready for the weights: keys that a column does not see are -inf, and the
+// references move up where one of them has to.  sk, lsv: this lane's block's K scale and log2 of its
+// V scale; qs: the columns' powers of two; lim: the last position each column sees; masked: some
+// column does not see all 32 keys.
+template <int kTiles>
+__device__ __forceinline__ void q8_references(f32x4_t (&s)[kTiles][2], float (&f)[kTiles], int key0, bool masked, float sk,
+                                              float lsv, const float (&qs)[kTiles], const int (&lim)[kTiles], int lane,
+                                              Q8State<kTiles>& st) {
+    const int g = lane >> 4;
+#pragma unroll
+    for (int c = 0; c < kTiles; ++c) f[c] = sk * qs[c];
+    if (masked) {
+#pragma unroll
+        for (int c = 0; c < kTiles; ++c) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                s[c][j >> 2][j & 3] = key0 + 8 * g + j <= lim[c] ? s[c][j >> 2][j & 3] * f[c] : -__builtin_inff();
+            f[c] = 1.0f;
+        }
+    }
+    float top[kTiles];
+    bool over = false;
 #pragma unroll
     for (int c = 0; c < kTiles; ++c) {
-        float x[8];
-        float f = sk * qs[c];
+        top[c] = max8(s[c]) * f[c];
+        over |= top[c] > st.m[c] + kSlack || top[c] + lsv > st.mv[c] + kSlack;
+    }
+    if (__any(over)) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = s[c][j >> 2][j & 3];
-        if (masked) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = key0 + 8 * g + j <= lim[c] ? x[j] * f : -__builtin_inff();
-            f = 1.0f;
-        }
-        float top = x[0];
-#pragma unroll
-        for (int j = 1; j < 8; ++j) top = fmaxf(top, x[j]);
-        top *= f;
-        const float m = swap32_max(swap16_max(fmaxf(st.m[c], top)));
-        const float mv = swap32_max(swap16_max(fmaxf(st.mv[c], top + lsv)));
-        // (a V scale 2^100 below the column's others': its weights are 0 in fp16 either way)
-        const float base = fminf(mv - lsv, m + 100.0f);
-        float sum = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j], f, -base));
-            sum += w;
-            p[c][j] = static_cast<_Float16>(w);
-        }
-        st.l[c] = st.l[c] * __builtin_amdgcn_exp2f(st.m[c] - m) + sum * __builtin_amdgcn_exp2f(base - m);
-        if (__any(mv > st.mv[c])) {
+        for (int c = 0; c < kTiles; ++c) {
+            const float m = swap32_max(swap16_max(fmaxf(st.m[c], top[c])));
+            const float mv = swap32_max(swap16_max(fmaxf(st.mv[c], top[c] + lsv)));
+            st.l[c] *= __builtin_amdgcn_exp2f(st.m[c] - m);
             const float down = __builtin_amdgcn_exp2f(st.mv[c] - mv);
 #pragma unroll
             for (int dt = 0; dt < 8; ++dt) st.o[c][dt] *= down;
+            st.m[c] = m;
+            st.mv[c] = mv;
         }
-        st.m[c] = m;
-        st.mv[c] = mv;
     }
-    // O^T += V^T P^T: A = 16 dims x 32 keys by transposed reads of V's rows.
-    const int vrow = 8 * g + (r >> 1);
-    const uint8_t* vrowp = vp + vrow * kQ8RowB + 8 * (r & 1);
+}
+
+// The lane's eight weights of a column as its B operand, and their part of the softmax sum.
+template <int kTiles>
+__device__ __forceinline__ q8_f16x8 q8_weights(const f32x4_t (&s)[2], float f, float lsv, int c, Q8State<kTiles>& st) {
+    // (a V scale 2^100 below the column's others': its weights are 0 in fp16 either way)
+    const float base = fminf(st.mv[c] - lsv, st.m[c] + 100.0f);
+    q8_f16x8 p;
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+        const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j >> 2][j & 3], f, -base));
+        const float w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j >> 2][(j & 3) + 1], f, -base));
+        const q8_f16x2 w = q8_pack(w0, w1);
+        p[j] = w.x;
+        p[j + 1] = w.y;
+        sum += w0 + w1;
+    }
+    st.l[c] = __builtin_fmaf(sum, __builtin_amdgcn_exp2f(base - st.m[c]), st.l[c]);
+    return p;
+}
+
+// O^T += V^T P^T: A = 16 dims x 32 keys.
+template <int kFmt, int kTiles>
+__device__ __forceinline__ void q8_values(const Q8VRows& v, const q8_f16x8 (&p)[kTiles], Q8State<kTiles>& st) {
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt) {
-        const q8_i32x2 v = __builtin_amdgcn_ds_read_tr8_b64_v2i32((q8_lds_i32x2*)(vrowp + 16 * (dt ^ v_swizzle(vrow))));
-        const q8_f16x8 av = q8_eight<kFmt>(static_cast<uint32_t>(v.x), static_cast<uint32_t>(v.y));
+        const q8_f16x8 av = q8_eight<kFmt>(static_cast<uint32_t>(v.w[dt].x), static_cast<uint32_t>(v.w[dt].y));
 #pragma unroll
         for (int c = 0; c < kTiles; ++c)
             st.o[c][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, p[c], st.o[c][dt], 0, 0, 0);
     }
 }
 
-// Block ids and scales of up to 64 blocks (32 steps) of one (sequence, KV head), in LDS.
+// Block ids and scales of a (sequence, KV head), 64 blocks (32 steps) at a time: a batch.  They are
+// copied into LDS ahead of their use, the ids a batch ahead, the scales when the batch's first step is
+// requested.
+static __device__ const float kNoScale = __builtin_nanf("");
+
 struct Q8Batch {
     int32_t id[kWave];
     float sk[kWave], sv[kWave];
 };
+typedef GQA_LDS Q8Batch q8_batch;
 
-// Fills `bt` for blocks j0 .. j0 + 63 of a sequence with n_blk blocks (past the last: the last).
-// An id outside the pool reads block 0 and has a NaN scale, as a block with a scale below zero or
-// NaN: the rows that attend to it are NaN.
-__device__ __forceinline__ void fill_batch(const Q8AttnArgs& a, const int32_t* table, int h, int j0, int n_blk, int lane,
-                                           Q8Batch& bt) {
-    const int32_t id = table[min(j0 + lane, n_blk - 1)];
-    const bool ok = id >= 0 && id < a.pool.n_blocks;
-    const int64_t at = (ok ? id : 0) * a.pool.scale_block_stride + h * a.pool.scale_head_stride;
-    const float sk = a.pool.k_scale[at], sv = a.pool.v_scale[at];
-    const float nan = __builtin_nanf("");
-    bt.id[lane] = ok ? id : 0;
-    bt.sk[lane] = ok && sk >= 0.0f && sv >= 0.0f ? sk : nan;               // (NaN scores make the whole row NaN)
-    bt.sv[lane] = __builtin_amdgcn_logf(ok && sv >= 0.0f ? sv : 0.0f);     // log2
+// The ids of batch n of the sequence with table row `table` and n_blk blocks (past the last: its id).
+__device__ __forceinline__ void request_ids(q8_batch* bt, const int32_t* table, int n, int n_blk, int lane) {
+    copy4(table + min(kWave * n + lane, n_blk - 1), (q8_lds*)bt->id);
 }
 
-// Where the stream's ranges and segments lie.  The stream is every sequence's steps for KV head 0,
-// then 1, ... laid end to end; sequences of more than kQ8StreamMax rows are not in it.
-__device__ __forceinline__ int stream_steps(const Q8AttnArgs& a, int b) {
-    Q8Seq s;
-    if (b >= a.batch || !q8_seq(a, b, s) || s.n > kQ8StreamMax) return 0;
-    return (s.start + s.n + kQ8Step - 1) / kQ8Step;
+// The scales of a batch whose ids have landed.  An id outside the pool becomes block 0 with a NaN scale:
+// the rows that attend to it are NaN.
+__device__ __forceinline__ void request_scales(q8_batch* bt, const Q8Pool& pool, int h, int lane) {
+    const int32_t id = bt->id[lane];
+    const bool ok = id >= 0 && id < pool.n_blocks;
+    if (!ok) bt->id[lane] = 0;
+    const int64_t at = id * pool.scale_block_stride + h * pool.scale_head_stride;
+    copy4(ok ? pool.k_scale + at : &kNoScale, (q8_lds*)bt->sk);
+    copy4(ok ? pool.v_scale + at : &kNoScale, (q8_lds*)bt->sv);
 }
 
-// Steps of the whole stream over one KV head.
-__device__ int64_t stream_total(const Q8AttnArgs& a, int lane) {
-    int64_t sum = 0;
-    for (int b = lane; b < a.batch; b += kWave) sum += stream_steps(a, b);
-    for (int d = 1; d < kWave; d <<= 1) sum += __shfl_xor(sum, d);
-    return sum;
+__device__ __forceinline__ int64_t batch_block(const q8_batch* bt, int step, int which) {
+    return __builtin_amdgcn_readfirstlane(bt->id[2 * (step & 31) + which]);
 }
 
-__device__ __forceinline__ int64_t uniform64(int64_t v) {
-    const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
-    const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(static_cast<uint64_t>(v) >> 32));
-    return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
+// K scale and log2 of the V scale of the lane's block (its keys are 8 (lane / 16) .. of the step).  A
+// scale that is negative or NaN makes scores NaN, and with them the rows that attend to it.
+__device__ __forceinline__ void batch_scales(const q8_batch* bt, int step, int lane, float& sk, float& lsv) {
+    const int at = 2 * (step & 31) + (lane >> 5);
+    const float k = bt->sk[at], v = bt->sv[at];
+    sk = k >= 0.0f && v >= 0.0f ? k : __builtin_nanf("");
+    lsv = __builtin_amdgcn_logf(v >= 0.0f ? v : 0.0f);
 }
 
-constexpr int kMinRange = 2;               // steps of the smallest range
+// Inclusive sum over the wave's lanes (DPP: rows of 16, then the rows' totals handed on).
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x111, 0xf, 0xf, true);      // row_shr:1
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x112, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x114, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x118, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x142, 0xa, 0xf, false);     // row_bcast:15 into rows 1, 3
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x143, 0xc, 0xf, false);     // row_bcast:31 into rows 2, 3
+    return x;
+}
 
-__device__ __forceinline__ int64_t range_steps(int64_t total, int waves) {
-    const int64_t per = (total + waves - 1) / waves;
-    return per < kMinRange ? kMinRange : per;
+__device__ __forceinline__ int lane_value(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
+
+// The stream: the steps of every sequence of at most kQ8StreamMax rows, laid end to end.  Each KV head
+// streams them by itself.  A window is 64 sequences of it, one in each lane.
+struct Q8Window {
+    int b0;
+    Q8Seq seq;                             // this lane's
+    int steps;                             // 0: not in the stream
+
+    __device__ __forceinline__ void load(const Q8AttnArgs& a, int first, int lane) {
+        b0 = first;
+        seq = Q8Seq{0, 0, 0};
+        steps = 0;
+        if (b0 + lane < a.batch && q8_seq(a, b0 + lane, seq) && seq.n <= kQ8StreamMax)
+            steps = (seq.start + seq.n + kQ8Step - 1) / kQ8Step;
+    }
+};
+
+// How the stream is cut.  Each sequence begins with `lead` positions that hold no step: what starting
+// a piece takes (4 us of 1.2 us a step), so that a range which crosses sequences has fewer steps.
+// Where sequences are many ranges long there is none: few ranges start one, and ranges that
+// divide a length evenly stay aligned with it.
+constexpr int kMinRange = 4;               // steps of the smallest range (below, counting and merging costs more)
+constexpr int kLead = 3;
+
+struct Q8Cut {
+    int64_t total, per;                    // the stream's length, a range's
+    int lead;
+
+    __device__ __forceinline__ Q8Cut(int64_t steps, int seqs, int ranges) {
+        lead = 4 * static_cast<int64_t>(seqs) > ranges && steps >= 8 * static_cast<int64_t>(ranges) ? kLead : 0;
+        total = steps + static_cast<int64_t>(lead) * seqs;
+        per = max((total + ranges - 1) / ranges, static_cast<int64_t>(kMinRange));
+    }
+    // The first and last range that hold steps of a sequence whose step 0 is at position x.
+    __device__ __forceinline__ int first_range(int64_t x) const { return static_cast<int>(x / per); }
+    __device__ __forceinline__ int last_range(int64_t x, int steps) const { return static_cast<int>((x + steps - 1) / per); }
+};
+
+// Partials that another workgroup of the same launch reads go past the L2s, each of which serves one
+// XCD: accesses of agent scope (sc1).  (A release fence would write back the whole L2; atomics of 8
+// bytes take a cycle of the address unit for each lane: 0.19 us a partial, these 0.02.)
+constexpr int kAgentScope = 16;
+
+struct Q8Shared {
+    __amdgpu_buffer_rsrc_t rows, ml;
+
+    __device__ __forceinline__ explicit Q8Shared(const Q8AttnArgs& a) {
+        const int n = static_cast<int>(2 * a.stream_waves * kGroup);       // partial rows of one-token calls
+        rows = __builtin_amdgcn_make_buffer_rsrc(a.part_o, 0, n * kD * 4, 0x00027000);
+        ml = __builtin_amdgcn_make_buffer_rsrc(a.part_ml, 0, n * 16, 0x00027000);
+    }
+    static __device__ __forceinline__ f32x4_t get(__amdgpu_buffer_rsrc_t r, int at) {
+        return __builtin_bit_cast(f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, kAgentScope));
+    }
+    static __device__ __forceinline__ void put(__amdgpu_buffer_rsrc_t r, int at, f32x4_t x) {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(q8_u32x4, x), r, at, 0, kAgentScope);
+    }
+};
+
+// NaN rows (of KV head h) for a sequence whose lengths break the rules, or that has more than max_new
+// rows; none where its offsets do.
+__device__ __forceinline__ void write_nan(const Q8AttnArgs& a, const Q8Seq& sq, int h, int lane, int first, int stride) {
+    if (sq.row0 < 0 || sq.n <= 0 || static_cast<int64_t>(sq.row0) + sq.n > a.n_tokens) return;
+    for (int t = first; t < sq.n; t += stride) {
+        uint32_t* row = reinterpret_cast<uint32_t*>(a.out) + ((static_cast<int64_t>(sq.row0) + t) * kHq + kGroup * h) * (kD / 2);
+        for (int i = lane; i < kGroup * kD / 2; i += kWave) row[i] = 0x7fc07fc0u;
+    }
 }
 
 __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
@@ -365,8 +519,8 @@ __device__ __forceinline__ void write_out(const Q8AttnArgs& a, const Q8Seq& sq, 
     }
 }
 
-// The same rows as a partial: slot * columns + column.
-template <int kTiles>
+// The same rows as partials, row0 + column.  kOne: for this launch's merge.
+template <int kTiles, bool kOne>
 __device__ __forceinline__ void write_partial(const Q8AttnArgs& a, int64_t row0, int tokens, int lane, Q8State<kTiles>& st) {
     const int g = lane >> 4;
 #pragma unroll
@@ -374,152 +528,336 @@ __device__ __forceinline__ void write_partial(const Q8AttnArgs& a, int64_t row0,
         const int col = 16 * c + (lane & 15);
         const float l = cross_row_sum(st.l[c]);
         if ((col >> 2) >= tokens) continue;
-        float* row = a.part_o + (row0 + col) * kD + 4 * g;
+        const f32x4_t ml = {st.m[c], st.mv[c], l, 0.0f};
 #pragma unroll
         for (int dt = 0; dt < 8; ++dt) {
             f32x4_t o = st.o[c][dt];
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[i] = (st.nan[c] >> (4 * dt + i)) & 1 ? __builtin_nanf("") : o[i];
-            *reinterpret_cast<f32x4_t*>(row + 16 * dt) = o;
+            if constexpr (kOne) Q8Shared::put(Q8Shared(a).rows, static_cast<int>(row0 + col) * kD * 4 + 16 * g + 64 * dt, o);
+            else *reinterpret_cast<f32x4_t*>(a.part_o + (row0 + col) * kD + 4 * g + 16 * dt) = o;
         }
-        if (g == 0) a.part_ml[row0 + col] = make_float4(st.m[c], st.mv[c], l, 0.0f);
+        if (g != 0) continue;
+        if constexpr (kOne) Q8Shared::put(Q8Shared(a).ml, static_cast<int>(row0 + col) * 16, ml);
+        else *reinterpret_cast<f32x4_t*>(a.part_ml + row0 + col) = ml;
     }
+}
+
+// The n partials of a single token's four rows (one KV head) by one wave: lane (c, i) has dims 8i ..
+// 8i + 7 of column c.  kBatch partials are in flight at once.  row_of(i): partial i's first row.
+template <typename RowOf>
+__device__ __forceinline__ void merge_token(const Q8AttnArgs& a, int n, RowOf row_of, uint16_t* out, int lane) {
+    constexpr int kBatch = 8;
+    const Q8Shared parts(a);
+    const int c = lane >> 4, i8 = 8 * (lane & 15);
+    float m = kLowest, mv = kLowest, l = 0.0f, o[8] = {};
+    for (int i0 = 0; i0 < n; i0 += kBatch) {
+        f32x4_t ml[kBatch], x[kBatch][2];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            const int row = row_of(min(i0 + j, n - 1)) + c;
+            ml[j] = Q8Shared::get(parts.ml, row * 16);
+            x[j][0] = Q8Shared::get(parts.rows, (row * kD + i8) * 4);
+            x[j][1] = Q8Shared::get(parts.rows, (row * kD + i8) * 4 + 16);
+        }
+        float top = m, topv = mv;
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {         // (a partial past the last is the last again, with no weight)
+            top = fmaxf(top, ml[j][0]);
+            topv = fmaxf(topv, ml[j][1]);
+        }
+        const float down = __builtin_amdgcn_exp2f(mv - topv);
+        l *= __builtin_amdgcn_exp2f(m - top);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) o[k] *= down;
+        m = top;
+        mv = topv;
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            const float some = i0 + j < n ? 1.0f : 0.0f;
+            const float f = some * __builtin_amdgcn_exp2f(ml[j][1] - mv);
+            l = __builtin_fmaf(ml[j][2], some * __builtin_amdgcn_exp2f(ml[j][0] - m), l);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                o[k] = __builtin_fmaf(x[j][0][k], f, o[k]);
+                o[4 + k] = __builtin_fmaf(x[j][1][k], f, o[4 + k]);
+            }
+        }
+    }
+    const float f = __builtin_amdgcn_exp2f(mv - m) / l;
+    *reinterpret_cast<uint4*>(out + c * kD + i8) =
+        make_uint4(bf16_pair(o[0] * f, o[1] * f), bf16_pair(o[2] * f, o[3] * f), bf16_pair(o[4] * f, o[5] * f),
+                   bf16_pair(o[6] * f, o[7] * f));
 }
 
 }  // namespace
 
 // ---------------------------------------------------------------------------------------------
-// Stream kernel: sequences of at most kQ8StreamMax new tokens.  The keys of every (sequence, KV
-// head) end to end, cut into equal ranges, one wave each; the part of a segment in a range is a
-// piece.  A piece that is a whole segment writes its rows; others leave partials for the
-// merge: slot 2w of the piece that enters range w from the one before, 2w + 1 of the one that
-// leaves it.
-template <int kFmt, int kTiles>
-__global__ __launch_bounds__(kWave) __attribute__((amdgpu_waves_per_eu(kTiles == 4 ? 1 : 2)))
+// Stream kernel: sequences of at most kQ8StreamMax new tokens.  Their keys end to end, cut into equal
+// ranges, one wave for each range and KV head; the part of a sequence in a range is a piece.  A piece
+// that is a whole sequence writes its rows; others leave partials for the merge: slot 2w of the piece
+// that enters wave w's range from the one before, 2w + 1 of the one that leaves it.
+//
+// With one new token for each sequence (kOne) the merge is part of this kernel: the last of a sequence's
+// pieces to be written, by a counter in the workspace that it puts back to zero, merges them all, and
+// lengths that break the rules get their NaN rows here.  Of more tokens' partials one wave would
+// read up to megabytes: they have a launch of their own.
+//
+// The eight waves of a range are neighbours, one on each XCD, and read the eight heads' parts of the
+// same blocks at about the same time: HBM sees blocks of 16 KB, not 2.
+template <int kFmt, int kTiles, bool kOne>
+__global__ __launch_bounds__(kWave) __attribute__((amdgpu_waves_per_eu(1)))
 void q8_stream_kernel(Q8AttnArgs a) {
-    __shared__ __align__(16) uint8_t s_ring[2][2][kQ8PlaneB];          // [buffer][K, V]
-    __shared__ Q8Batch s_batch;
+    constexpr int kRing = q8_ring(kTiles);
+    constexpr int kCopies = 8;                     // memory operations of a step's copies
+    constexpr int kBatches = kRing + 1;            // the work's, up to kRing - 1 after it, and the next ids
+    __shared__ __align__(4096) uint8_t s_ring[kRing][2][kQ8PlaneB];    // [buffer][K, V]
+    __shared__ Q8Batch s_batch[kBatches];
     __shared__ float2 s_cs[kTiles * 4 * kPairs];
+    q8_lds* const ring = (q8_lds*)&s_ring[0][0][0];
+    q8_batch* const batches = (q8_batch*)&s_batch[0];
     const int lane = threadIdx.x;
-    const int64_t per_head = uniform64(stream_total(a, lane));
-    const int64_t total = per_head * kHkv;
-    const int64_t per = range_steps(total, a.stream_waves);
-    const int64_t wave = blockIdx.x;
-    int64_t x = wave * per;
-    const int64_t x_end = min(x + per, total);
-    if (x >= x_end) return;
+    const int wave = blockIdx.x;
+    const int h = wave % kHkv;
 
-    // The sequence that holds x: windows of 64 sequences.
-    int b = 0, steps = 0;
-    int64_t off = 0;                               // stream position of sequence b's first segment
+    // The stream's length, and the sequence at this wave's first position (one window in most batches).
+    Q8Window win;
+    int64_t all = 0;
+    int seqs = 0;
     for (int b0 = 0; b0 < a.batch; b0 += kWave) {
-        const int mine = stream_steps(a, b0 + lane);
-        int64_t upto = static_cast<int64_t>(mine) * kHkv;
-        for (int d = 1; d < kWave; d <<= 1) {
-            const int64_t y = __shfl_up(upto, d);
-            if (lane >= d) upto += y;
+        win.load(a, b0, lane);
+        all += static_cast<uint32_t>(lane_value(wave_scan(win.steps), kWave - 1));
+        seqs += __popcll(__ballot(win.steps > 0));
+        if constexpr (kOne) {                      // the wave of (b, h): b by the ranges in turn
+            uint64_t bad = __ballot(win.steps == 0 && win.seq.n > 0);
+            for (; bad; bad &= bad - 1) {
+                const int at = __builtin_ctzll(bad);
+                if ((b0 + at) % (a.stream_waves / kHkv) != wave / kHkv) continue;
+                write_nan(a, Q8Seq{lane_value(win.seq.row0, at), lane_value(win.seq.n, at), 0}, h, lane, 0, 1);
+            }
         }
-        const uint64_t past = __ballot(off + upto > x);
-        if (past) {
-            const int at = __builtin_ctzll(past);
-            b = b0 + at;
-            steps = __builtin_amdgcn_readfirstlane(__shfl(mine, at));
-            off += uniform64(__shfl(upto, at)) - static_cast<int64_t>(steps) * kHkv;
-            break;
-        }
-        off += uniform64(__shfl(upto, kWave - 1));
     }
-    b = __builtin_amdgcn_readfirstlane(b);
-    if (steps == 0) return;
-    int h = static_cast<int>((x - off) / steps);
-    int first = static_cast<int>((x - off) - static_cast<int64_t>(h) * steps);
+    const Q8Cut cut(all, seqs, a.stream_waves / kHkv);
+    int64_t x = wave / kHkv * cut.per;             // next position
+    const int64_t x_end = min(x + cut.per, cut.total);
+    if (x >= x_end) return;
+    int64_t off = 0;                               // position of the window's first sequence
+    if (win.b0) win.load(a, 0, lane);
+    uint32_t upto = wave_scan(win.steps > 0 ? win.steps + cut.lead : 0);
+    uint64_t past;
+    while (!(past = __ballot(off + upto > x))) {
+        off += static_cast<uint32_t>(lane_value(upto, kWave - 1));
+        if (win.b0 + kWave >= a.batch) return;     // (lengths that changed under the call)
+        win.load(a, win.b0 + kWave, lane);
+        upto = wave_scan(win.steps > 0 ? win.steps + cut.lead : 0);
+    }
 
-    uint32_t koff[4], voff[4];                     // this lane's part of a plane's copies, inside its block
+    // A piece: steps [first, end) of sequence b.  x moves past it.
+    struct Piece {
+        int b, row0, n, start, first, end, steps;
+        int64_t at;                                // position of its sequence's step 0
+    };
+    auto piece_at = [&](int at, int64_t skip) {    // `skip`: positions of the sequence before x
+        Piece p;
+        p.at = x - skip + cut.lead;
+        p.b = win.b0 + at;
+        p.row0 = lane_value(win.seq.row0, at);
+        p.n = lane_value(win.seq.n, at);
+        p.start = lane_value(win.seq.start, at);
+        p.steps = lane_value(win.steps, at);
+        p.first = static_cast<int>(max(skip - cut.lead, int64_t{0}));
+        const int64_t length = p.steps + cut.lead - skip;
+        p.end = static_cast<int>(max(min(x_end - x, length) + skip - cut.lead, int64_t{0}));
+        x += length;
+        return p;
+    };
+    // The piece behind p; one without steps where the range ends before it.
+    auto piece_after = [&](const Piece& p) {
+        uint64_t left = __ballot(win.steps > 0) & ~((2ull << (p.b - win.b0)) - 1);
+        while (!left && win.b0 + kWave < a.batch) {
+            win.load(a, win.b0 + kWave, lane);
+            left = __ballot(win.steps > 0);
+        }
+        return piece_at(left ? __builtin_ctzll(left) : 0, 0);
+    };
+    const int at0 = __builtin_ctzll(past);
+    Piece cur = piece_at(at0, x - off - static_cast<uint32_t>(lane_value(upto, at0)) + lane_value(win.steps, at0) + cut.lead);
+    if (cur.first == cur.end) {                    // the range begins with positions that hold no step
+        if (x >= x_end) return;
+        cur = piece_after(cur);
+        if (cur.first == cur.end) return;
+    }
+
+    uint32_t kcopy[4], vcopy[4];                   // this lane's part of a plane's copies, inside its block
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
         const int row = copy_row(q, lane);
         const uint32_t at = static_cast<uint32_t>((row & 15) * a.pool.pos_stride);
-        koff[q] = at + 16u * ((lane & 7) ^ k_swizzle(row));
-        voff[q] = at + 16u * ((lane & 7) ^ v_swizzle(row));
+        kcopy[q] = at + 16u * ((lane & 7) ^ k_swizzle(row));
+        vcopy[q] = at + 16u * ((lane & 7) ^ v_swizzle(row));
     }
+    const uint32_t koff = k_offset(lane), voff = v_offset(lane);
+    const uint8_t* kh = a.pool.k + h * a.pool.head_stride;
+    const uint8_t* vh = a.pool.v + h * a.pool.head_stride;
 
+    // Requests run up to kRing - 1 steps ahead of the work, into the next piece too.  Both sides take the
+    // batches in the same order, in the slots of s_batch in turn.
+    Piece feed = cur, next = cur;                  // the piece requests are made for; the piece after cur
+    bool have_next = x < x_end, feed_next = false; // feed is `next`
+    if (have_next) {
+        next = piece_after(cur);
+        have_next = next.end > 0;
+    }
+    int feed_step = cur.first, batch_end = cur.first;      // the next step to request; where its batch ends
+    int feed_slot = kBatches - 1, feed_buf = 0, ahead = 0;
+    bool ids_due = false;                          // the ids of the next batch are not requested: its piece is not known yet
+    int since = 0;                                 // steps requested since the last ids were
+    auto following = [](int slot) { return slot + 1 == kBatches ? 0 : slot + 1; };
+    auto ids = [&](const Piece& p, int n) {
+        request_ids(batches + following(feed_slot), a.block_table + static_cast<int64_t>(p.b) * a.max_blocks, n,
+                    (p.start + p.n - 1) / kQ8Block + 1, lane);
+        since = 0;
+    };
+    auto request = [&]() {
+        if (feed_step == batch_end) {
+            if (feed_step == feed.end) {
+                if (!have_next || feed_next) return false;
+                feed = next;
+                feed_next = true;
+                feed_step = 0;
+            }
+            if (since >= 2) wait_copies<2 * kCopies>();    // the ids have landed
+            else if (since == 1) wait_copies<kCopies>();
+            else wait_copies<0>();
+            feed_slot = following(feed_slot);
+            request_scales(batches + feed_slot, a.pool, h, lane);
+            const int n = feed_step / 32 + 1;
+            batch_end = min(32 * n, feed.end);
+            ids_due = false;
+            if (32 * n < feed.end) ids(feed, n);
+            else if (have_next && !feed_next) ids(next, 0);
+            else ids_due = true;
+        }
+        const q8_batch* bt = batches + feed_slot;
+        const int64_t id0 = batch_block(bt, feed_step, 0), id1 = batch_block(bt, feed_step, 1);
+        q8_lds* dst = ring + feed_buf * 2 * kQ8PlaneB;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+            const uint8_t* base = kv ? vh : kh;
+            const uint8_t* b0 = base + id0 * a.pool.block_stride;
+            const uint8_t* b1 = base + id1 * a.pool.block_stride;
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                copy16<true>(q < 2 ? b0 : b1, (kv ? vcopy : kcopy)[q], dst + kv * kQ8PlaneB + q * 1024);
+        }
+        feed_buf = feed_buf + 1 == kRing ? 0 : feed_buf + 1;
+        ++feed_step;
+        ++ahead;
+        ++since;
+        return true;
+    };
+
+    auto wait_steps = [&](int left) {              // until at most `left` steps' copies are in flight
+        if (kRing > 3 && left >= 3) wait_copies<3 * kCopies>();
+        else if (kRing > 2 && left >= 2) wait_copies<2 * kCopies>();
+        else if (left >= 1) wait_copies<kCopies>();
+        else wait_copies<0>();
+    };
+
+    // The wave's unfinished sequences (kOne): the one its range begins inside of, and the one it ends in.
+    struct Part {
+        int b, row0, r0, n;                        // the first of the sequence's n pieces is of range r0; n = 0: none
+    };
+    Part entering{0, 0, 0, 0}, leaving{0, 0, 0, 0};
+
+    ids(cur, cur.first / 32);
+    int slot = 0, buf = 0;
     Q8State<kTiles> st;
-    q8_f16x8 qop[kTiles][4];
-    float qs[kTiles];
-    int lim[kTiles];
     while (true) {
-        Q8Seq sq;
-        q8_seq(a, b, sq);
-        sq.row0 = __builtin_amdgcn_readfirstlane(sq.row0);
-        sq.n = __builtin_amdgcn_readfirstlane(sq.n);
-        sq.start = __builtin_amdgcn_readfirstlane(sq.start);
-        const int n_steps = static_cast<int>(min(static_cast<int64_t>(steps - first), x_end - x));
-        const int end = first + n_steps;
-        const int last = sq.start + sq.n - 1;
-        const int n_blk = last / kQ8Block + 1;
-        const int32_t* table = a.block_table + static_cast<int64_t>(b) * a.max_blocks;
-        const uint8_t* kh = a.pool.k + h * a.pool.head_stride;
-        const uint8_t* vh = a.pool.v + h * a.pool.head_stride;
-
-        auto issue = [&](int step, int buf) {
-#pragma unroll
-            for (int kv = 0; kv < 2; ++kv)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int64_t id = __builtin_amdgcn_readfirstlane(s_batch.id[2 * (step & 31) + (q >> 1)]);
-                    copy16((kv ? vh : kh) + id * a.pool.block_stride, (kv ? voff : koff)[q], s_ring[buf][kv] + q * 1024, true);
-                }
-        };
-
-        fill_batch(a, table, h, 2 * (first & ~31), n_blk, lane, s_batch);
-        __syncthreads();
-        issue(first, first & 1);
-        fill_angles(a, sq.start, sq.n, s_cs, lane, kWave);
-        __syncthreads();
+        Q8Row raw[kTiles];
 #pragma unroll
         for (int c = 0; c < kTiles; ++c) {
-            const int col = 16 * c + (lane & 15), tok = min(col >> 2, sq.n - 1);
-            qs[c] = load_q(a, a.q + static_cast<int64_t>(sq.row0 + tok) * a.q_token_stride + (kGroup * h + (col & 3)) * kD,
-                           s_cs + tok * kPairs, lane >> 4, qop[c]);
-            lim[c] = sq.start + tok;
+            const int col = 16 * c + (lane & 15);
+            raw[c] = fetch_q(q_row(a, cur.row0 + min(col >> 2, cur.n - 1), h, col & 3), lane >> 4);
+        }
+        while (ahead < kRing - 1 && request()) {}
+        fill_angles(a, cur.start, cur.n, s_cs, lane, kWave);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        q8_f16x8 qop[kTiles][4];
+        float qs[kTiles];
+        int lim[kTiles];
+#pragma unroll
+        for (int c = 0; c < kTiles; ++c) {
+            const int tok = min((16 * c + (lane & 15)) >> 2, cur.n - 1);
+            qs[c] = make_q(a, raw[c], s_cs + tok * kPairs, lane >> 4, qop[c]);
+            lim[c] = cur.start + tok;
         }
         st.clear();
-        for (int step = first; step < end; ++step) {
-            const int j = 2 * (step & 31) + (lane >> 5);
-            const float sk = s_batch.sk[j], lsv = s_batch.sv[j];
-            if (step + 1 < end) {
-                if (((step + 1) & 31) == 0) {
-                    __syncthreads();
-                    fill_batch(a, table, h, 2 * (step + 1), n_blk, lane, s_batch);
-                    __syncthreads();
-                }
-                issue(step + 1, (step + 1) & 1);
-                wait_copies<8>();
-            } else {
-                wait_copies<0>();
-            }
+        for (int step = cur.first; step < cur.end; ++step) {
+            request();
+            wait_steps(ahead - 1);
+            const q8_lds* kp = ring + buf * 2 * kQ8PlaneB;
+            q8_lds* vp = ring + buf * 2 * kQ8PlaneB + kQ8PlaneB;
+            buf = buf + 1 == kRing ? 0 : buf + 1;
             const int key0 = step * kQ8Step;
-            const bool masked = key0 + kQ8Step - 1 > sq.start;
-            if (masked) mask_values<kFmt, kTiles>(s_ring[step & 1][1], key0, last, lim, lane, kWave, st);
-            q8_step<kFmt, kTiles>(s_ring[step & 1][0], s_ring[step & 1][1], key0, masked, sk, lsv, qop, qs, lim, lane, st);
+            const bool masked = key0 + kQ8Step - 1 > cur.start;
+            if (masked) mask_values<kFmt, kTiles>(vp, key0, cur.start + cur.n - 1, lim, lane, kWave, st);
+            const Q8KRows k = read_keys(kp, koff);
+            float sk, lsv;
+            batch_scales(batches + slot, step, lane, sk, lsv);
+            const Q8VRows v = read_values(vp, voff);
+            __builtin_amdgcn_sched_barrier(0);
+            f32x4_t s[kTiles][2];
+            q8_scores<kFmt, kTiles>(k, qop, s);
+            float f[kTiles];
+            q8_references<kTiles>(s, f, key0, masked, sk, lsv, qs, lim, lane, st);
+            q8_f16x8 p[kTiles];
+#pragma unroll
+            for (int c = 0; c < kTiles; ++c) p[c] = q8_weights<kTiles>(s[c], f[c], lsv, c, st);
+            q8_values<kFmt, kTiles>(v, p, st);
+            if ((step & 31) == 31 || step + 1 == cur.end) slot = following(slot);
+            --ahead;
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // the buffer's reads are done before it is refilled
         }
-        if (first == 0 && end == steps)
+        const Q8Seq sq{cur.row0, cur.n, cur.start};
+        if (cur.first == 0 && cur.end == cur.steps) {
             write_out<kTiles>(a, sq, 0, h, lane, st);
-        else
-            write_partial<kTiles>(a, (2 * wave + (first == 0 ? 1 : 0)) * (16 * kTiles), sq.n, lane, st);
-        x += n_steps;
-        if (x >= x_end) break;
-        first = 0;
-        if (++h == kHkv) {
-            h = 0;
-            do {
-                ++b;
-                steps = __builtin_amdgcn_readfirstlane(stream_steps(a, b));
-            } while (steps == 0 && b < a.batch);
-            if (steps == 0) break;                 // (lengths that changed under the call)
+        } else {
+            constexpr int kCols = kOne ? kGroup : 16 * kTiles;
+            write_partial<kTiles, kOne>(a, (2 * static_cast<int64_t>(wave) + (cur.first == 0 ? 1 : 0)) * kCols, cur.n, lane, st);
+            if constexpr (kOne) {                  // counted when the wave has no more to request
+                const int r0 = cut.first_range(cur.at), n = cut.last_range(cur.at, cur.steps) - r0 + 1;
+                (cur.first == 0 ? leaving : entering) = Part{cur.b, cur.row0, r0, n};
+            }
         }
-        __syncthreads();
+        if (!have_next) break;
+        cur = next;                                // (which the last request has entered: feed is `cur` now)
+        feed_next = false;
+        have_next = x < x_end;
+        if (have_next) {
+            next = piece_after(cur);
+            have_next = next.end > 0;
+        }
+        if (have_next && ids_due) ids(next, 0);
+        ids_due = false;
+    }
+    if constexpr (kOne) {
+        if (entering.n == 0 && leaving.n == 0) return;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");               // the partials are written before they count
+        const Part mine = lane == 0 ? entering : leaving;
+        uint32_t* counter = a.counters + h * kQ8MaxBatch + mine.b;
+        uint32_t done = 0;
+        if (lane < 2 && mine.n) done = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1;
+        uint64_t last = __ballot(lane < 2 && mine.n && done == static_cast<uint32_t>(mine.n));
+        asm volatile("" ::: "memory");
+        if ((last >> lane) & 1) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        for (; last; last &= last - 1) {
+            const Part part = (last & 1) ? entering : leaving;
+            auto row_of = [&](int i) {
+                return (2 * ((part.r0 + i) * kHkv + h) + (i == 0 ? 1 : 0)) * kGroup;
+            };
+            merge_token(a, part.n, row_of, a.out + (static_cast<int64_t>(part.row0) * kHq + kGroup * h) * kD, lane);
+        }
     }
 }
 
@@ -579,21 +917,23 @@ __device__ __forceinline__ int run_steps(int steps, int runs) { return max(kTile
 
 template <int kFmt>
 __global__ __launch_bounds__(kTileWaves * kWave) void q8_tile_kernel(Q8AttnArgs a) {
-    __shared__ __align__(16) uint8_t s_ring[2][2][kQ8PlaneB];
-    __shared__ Q8Batch s_batch;
-    __shared__ float2 s_cs[kQ8TileTokens * kPairs];
     constexpr int kTiles = 4;
+    __shared__ __align__(4096) uint8_t s_ring[2][2][kQ8PlaneB];
+    __shared__ Q8Batch s_batch[kTileWaves][2];     // (a copy for each wave: no barrier for them)
+    __shared__ float2 s_cs[kQ8TileTokens * kPairs];
     const int lane = threadIdx.x & (kWave - 1);
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    q8_lds* const ring = (q8_lds*)&s_ring[0][0][0];
     const int tiles = count_tiles(a, lane);
     const int runs = tile_runs(tiles, a.tile_wgs);
-    uint32_t koff, voff;
+    uint32_t kcopy, vcopy;
     {
         const int row = copy_row(wv, lane);
         const uint32_t at = static_cast<uint32_t>((row & 15) * a.pool.pos_stride);
-        koff = at + 16u * ((lane & 7) ^ k_swizzle(row));
-        voff = at + 16u * ((lane & 7) ^ v_swizzle(row));
+        kcopy = at + 16u * ((lane & 7) ^ k_swizzle(row));
+        vcopy = at + 16u * ((lane & 7) ^ v_swizzle(row));
     }
+    const uint32_t koff = k_offset(lane), voff = v_offset(lane);
     const int64_t items = static_cast<int64_t>(tiles) * kHkv * runs;
     for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
         const int h = static_cast<int>(item % kHkv);
@@ -615,18 +955,28 @@ __global__ __launch_bounds__(kTileWaves * kWave) void q8_tile_kernel(Q8AttnArgs 
         if (first >= end) continue;
         const int n_blk = last / kQ8Block + 1;
         const int32_t* table = a.block_table + static_cast<int64_t>(b) * a.max_blocks;
+        q8_batch* const batches = (q8_batch*)&s_batch[wv][0];
         const uint8_t* kh = a.pool.k + h * a.pool.head_stride;
         const uint8_t* vh = a.pool.v + h * a.pool.head_stride;
-        auto issue = [&](int step, int buf) {
-            const int64_t id = __builtin_amdgcn_readfirstlane(s_batch.id[2 * (step & 31) + (wv >> 1)]);
-            copy16(kh + id * a.pool.block_stride, koff, s_ring[buf][0] + wv * 1024, false);
-            copy16(vh + id * a.pool.block_stride, voff, s_ring[buf][1] + wv * 1024, false);
+        auto request = [&](int step) {
+            if ((step & 31) == 0 && step != first) {
+                wait_copies<0>();
+                request_scales(batches + ((step >> 5) & 1), a.pool, h, lane);
+                request_ids(batches + (~(step >> 5) & 1), table, (step >> 5) + 1, n_blk, lane);
+            }
+            const int64_t at = batch_block(batches + ((step >> 5) & 1), step, wv >> 1) * a.pool.block_stride;
+            q8_lds* dst = ring + (step & 1) * 2 * kQ8PlaneB + wv * 1024;
+            copy16<false>(kh + at, kcopy, dst);
+            copy16<false>(vh + at, vcopy, dst + kQ8PlaneB);
         };
-        __syncthreads();
-        if (wv == 0) fill_batch(a, table, h, 2 * (first & ~31), n_blk, lane, s_batch);
+        request_ids(batches + ((first >> 5) & 1), table, first >> 5, n_blk, lane);
+        __syncthreads();                           // (the item before is done with the ring and the angles)
         fill_angles(a, sq.start + tok0, tokens, s_cs, threadIdx.x, kTileWaves * kWave);
+        wait_copies<0>();
+        request_scales(batches + ((first >> 5) & 1), a.pool, h, lane);
+        request_ids(batches + (~(first >> 5) & 1), table, (first >> 5) + 1, n_blk, lane);
+        request(first);
         __syncthreads();
-        issue(first, first & 1);
         Q8State<kTiles> st;
         q8_f16x8 qop[kTiles][4];
         float qs[kTiles];
@@ -634,39 +984,45 @@ __global__ __launch_bounds__(kTileWaves * kWave) void q8_tile_kernel(Q8AttnArgs 
 #pragma unroll
         for (int c = 0; c < kTiles; ++c) {
             const int col = 16 * c + (lane & 15), tok = min(16 * wv + (col >> 2), tokens - 1);
-            qs[c] = load_q(a, a.q + static_cast<int64_t>(sq.row0 + tok0 + tok) * a.q_token_stride + (kGroup * h + (col & 3)) * kD,
-                           s_cs + tok * kPairs, lane >> 4, qop[c]);
+            const Q8Row raw = fetch_q(q_row(a, sq.row0 + tok0 + tok, h, col & 3), lane >> 4);
+            qs[c] = make_q(a, raw, s_cs + tok * kPairs, lane >> 4, qop[c]);
             lim[c] = sq.start + tok0 + tok;
         }
         st.clear();
         for (int step = first; step < end; ++step) {
-            const int j = 2 * (step & 31) + (lane >> 5);
-            const float sk = s_batch.sk[j], lsv = s_batch.sv[j];
             wait_copies<0>();
             __syncthreads();                       // the step has landed, and the other buffer is free
-            if (step + 1 < end) {
-                if (((step + 1) & 31) == 0) {
-                    if (wv == 0) fill_batch(a, table, h, 2 * (step + 1), n_blk, lane, s_batch);
-                    __syncthreads();
-                }
-                issue(step + 1, (step + 1) & 1);
-            }
+            if (step + 1 < end) request(step + 1);
+            float sk, lsv;
+            batch_scales(batches + ((step >> 5) & 1), step, lane, sk, lsv);
             const int key0 = step * kQ8Step;
             const bool masked = key0 + kQ8Step - 1 > sq.start + tok0;
-            if (masked) mask_values<kFmt, kTiles>(s_ring[step & 1][1], key0, last, lim, threadIdx.x, kTileWaves * kWave, st);
-            q8_step<kFmt, kTiles>(s_ring[step & 1][0], s_ring[step & 1][1], key0, masked, sk, lsv, qop, qs, lim, lane, st);
+            q8_lds* kp = ring + (step & 1) * 2 * kQ8PlaneB;
+            if (masked) mask_values<kFmt, kTiles>(kp + kQ8PlaneB, key0, last, lim, threadIdx.x, kTileWaves * kWave, st);
+            f32x4_t s[kTiles][2];
+            float f[kTiles];
+            const Q8KRows k = read_keys(kp, koff);
+            const Q8VRows v = read_values(kp + kQ8PlaneB, voff);
+            __builtin_amdgcn_sched_barrier(0);
+            q8_scores<kFmt, kTiles>(k, qop, s);
+            q8_references<kTiles>(s, f, key0, masked, sk, lsv, qs, lim, lane, st);
+            q8_f16x8 p[kTiles];
+#pragma unroll
+            for (int c = 0; c < kTiles; ++c) p[c] = q8_weights<kTiles>(s[c], f[c], lsv, c, st);
+            q8_values<kFmt, kTiles>(v, p, st);
         }
+        wait_copies<0>();
         if (per >= steps) {
             write_out<kTiles>(a, sq, tok0 + 16 * wv, h, lane, st);
         } else {
             const int64_t slot = (static_cast<int64_t>(tile) * kHkv + h) * runs + run;
-            write_partial<kTiles>(a, a.tile_slot0 + slot * kTileCols + 64 * wv, tokens - 16 * wv, lane, st);
+            write_partial<kTiles, false>(a, a.tile_slot0 + slot * kTileCols + 64 * wv, tokens - 16 * wv, lane, st);
         }
     }
 }
 
 // ---------------------------------------------------------------------------------------------
-// Merge: out = sum_i O_i 2^(M_i - m) / sum_i l_i 2^(m_i - m) over the partials of a row, and NaN
+// Merge kernels: out = sum_i O_i 2^(M_i - m) / sum_i l_i 2^(m_i - m) over the partials of a row, and NaN
 // rows for sequences whose lengths break the rules.
 namespace {
 
@@ -704,34 +1060,35 @@ __global__ __launch_bounds__(kGroup * kWave) void q8_stream_merge_kernel(Q8AttnA
     const int b = blockIdx.x / kHkv, h = blockIdx.x % kHkv;
     Q8Seq sq;
     if (!q8_seq(a, b, sq)) {
-        // Rows of a sequence whose lengths break the rules (or that has more than max_new): NaN.
-        if (sq.row0 < 0 || sq.n <= 0 || static_cast<int64_t>(sq.row0) + sq.n > a.n_tokens) return;
-        for (int t = blockIdx.y; t < sq.n; t += gridDim.y)
-            reinterpret_cast<uint32_t*>(a.out)[((static_cast<int64_t>(sq.row0) + t) * kHq + kGroup * h + head) * (kD / 2) + lane] =
-                0x7fc07fc0u;
+        if (head == 0) write_nan(a, sq, h, lane, blockIdx.y, gridDim.y);
         return;
     }
     const int tok = blockIdx.y;
     if (sq.n > kQ8StreamMax || tok >= sq.n) return;
     // The segment's place in the stream.
-    int64_t off = 0, all = 0;
-    for (int i = lane; i < a.batch; i += kWave) {
-        const int s = stream_steps(a, i);
-        all += s;
-        off += i < b ? s : 0;
+    int64_t before = 0, all = 0;
+    int steps = 0, seqs = 0, seqs_before = 0;
+    Q8Window win;
+    for (int b0 = 0; b0 < a.batch; b0 += kWave) {
+        win.load(a, b0, lane);
+        const uint32_t upto = wave_scan(win.steps);
+        const uint64_t some = __ballot(win.steps > 0);
+        if (b - b0 >= 0 && b - b0 < kWave) {
+            steps = lane_value(win.steps, b - b0);
+            before = all + static_cast<uint32_t>(lane_value(upto, b - b0)) - steps;
+            seqs_before = seqs + __popcll(some & ((1ull << (b - b0)) - 1));
+        }
+        all += static_cast<uint32_t>(lane_value(upto, kWave - 1));
+        seqs += __popcll(some);
     }
-    for (int d = 1; d < kWave; d <<= 1) {
-        all += __shfl_xor(all, d);
-        off += __shfl_xor(off, d);
-    }
-    const int steps = stream_steps(a, b);
-    const int64_t per = range_steps(uniform64(all) * kHkv, a.stream_waves);
-    const int64_t x = uniform64(off) * kHkv + static_cast<int64_t>(h) * steps;
-    const int64_t w0 = x / per, w1 = (x + steps - 1) / per;
-    if (w0 == w1) return;                          // one piece: written already
+    if (steps == 0) return;
+    const Q8Cut cut(all, seqs, a.stream_waves / kHkv);
+    const int64_t x = before + static_cast<int64_t>(cut.lead) * (seqs_before + 1);
+    const int64_t r0 = cut.first_range(x), r1 = cut.last_range(x, steps);
+    if (r0 == r1) return;                          // one piece: written already
     const int col = kGroup * tok + head;
-    merge_row(a, 2 * (w0 + 1) * cols + col, (2 * w0 + 1) * cols + col, 2 * cols, static_cast<int>(w1 - w0 + 1),
-              a.out + (static_cast<int64_t>(sq.row0 + tok) * kHq + kGroup * h + head) * kD, lane);
+    merge_row(a, 2 * ((r0 + 1) * kHkv + h) * cols + col, (2 * (r0 * kHkv + h) + 1) * cols + col, 2 * kHkv * cols,
+              static_cast<int>(r1 - r0 + 1), a.out + (static_cast<int64_t>(sq.row0 + tok) * kHq + kGroup * h + head) * kD, lane);
 }
 
 // Grid: workgroups of the tile kernel, tokens of a tile.
@@ -757,13 +1114,18 @@ __global__ __launch_bounds__(kGroup * kWave) void q8_tile_merge_kernel(Q8AttnArg
               a.out + (static_cast<int64_t>(sq.row0 + t) * kHq + kGroup * h + head) * kD, lane);
 }
 
-template <int kFmt, int kTiles>
+template <int kFmt, int kTiles, bool kOne = false>
 static void launch_stream(const Q8AttnArgs& a, hipStream_t stream) {
-    hipLaunchKernelGGL((q8_stream_kernel<kFmt, kTiles>), dim3(static_cast<unsigned>(a.stream_waves)), dim3(kWave), 0, stream, a);
+    hipLaunchKernelGGL((q8_stream_kernel<kFmt, kTiles, kOne>), dim3(static_cast<unsigned>(a.stream_waves)), dim3(kWave), 0,
+                       stream, a);
 }
 
 template <int kFmt>
 static hipError_t launch_attention(const Q8AttnArgs& a, hipStream_t stream) {
+    if (a.max_new == 1) {
+        launch_stream<kFmt, 1, true>(a, stream);
+        return hipGetLastError();
+    }
     const int tiles = q8_stream_tiles(a.max_new);
     if (a.max_new > kQ8StreamMax)
         hipLaunchKernelGGL((q8_tile_kernel<kFmt>), dim3(static_cast<unsigned>(a.tile_wgs)), dim3(kTileWaves * kWave), 0, stream, a);

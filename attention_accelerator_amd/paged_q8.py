@@ -17,9 +17,19 @@ import torch
 
 from . import _lib
 from ._lib import GQA_Q8_E4M3, GQA_Q8_INT8, GqaParams, GqaQ8Kv, check, lib
-from .attention import BLOCK_SIZE, HEAD_DIM, N_KV_HEADS, N_Q_HEADS, ROPE_THETA, _stream_handle, make_params
+from .attention import BLOCK_SIZE, HEAD_DIM, N_KV_HEADS, N_Q_HEADS, ROPE_THETA, make_params
 
 Q8_FORMATS = {torch.int8: GQA_Q8_INT8, torch.float8_e4m3fn: GQA_Q8_E4M3}
+
+
+def _call(fn, device: torch.device, *args) -> int:
+    """fn(*args, the current stream of `device`) with that device current.  (The raw handle: a
+    torch.cuda.Stream object for it takes 2 us, a small call's kernel 5.)"""
+    index = device.index
+    if torch.cuda.current_device() == index:
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
 
 
 class Q8Pool(NamedTuple):
@@ -72,9 +82,12 @@ def _table(t: torch.Tensor, device, batch: int) -> torch.Tensor:
     return t
 
 
-def _overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
-    ends = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in (a, b)]
-    return max(ends[0][0], ends[1][0]) < min(ends[0][1], ends[1][1])
+def _span(t: torch.Tensor):
+    """The addresses that an int32 tensor's elements lie in: [first, end)."""
+    start = t.data_ptr()
+    if t.is_contiguous():
+        return start, start + 4 * t.numel()
+    return start, start + 4 * (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride())))
 
 
 def paged_plan(cached: torch.Tensor, n_new: torch.Tensor, free_blocks: torch.Tensor, n_free: torch.Tensor,
@@ -103,41 +116,45 @@ def paged_plan(cached: torch.Tensor, n_new: torch.Tensor, free_blocks: torch.Ten
     n_rows = int(n_rows)
     sizes = (batch, batch + 1, n_rows, n_rows, 1)
     if out is None:
-        out = PagedPlan(*(torch.empty(max(n, 0), dtype=torch.int32, device=device) for n in sizes))
+        if n_rows < 0 or batch == 0:
+            check(_lib.GQA_ERR_INVALID_CONFIG, "gqa_paged_plan")
+        out = PagedPlan(*torch.empty(sum(sizes), dtype=torch.int32, device=device).split_with_sizes(sizes))
     else:
+        inputs = [_span(t) for t in (cached, n_new, free_blocks, n_free, block_table)]
         for t, n, name in zip(out, sizes, PagedPlan._fields):
-            _int32(t, f"out.{name}", device, n)
-            for given in (cached, n_new, free_blocks, n_free, block_table):
-                if _overlaps(t, given):
+            lo = _int32(t, name, device, n).data_ptr()
+            hi = lo + 4 * n
+            for first, end in inputs:
+                if lo < end and first < hi:
                     raise ValueError(f"out.{name} overlaps an input")
-    with torch.cuda.device(device):
-        status = lib().gqa_paged_plan(cached.data_ptr(), n_new.data_ptr(), batch, free_blocks.data_ptr(),
-                                      n_free.data_ptr(), free_blocks.numel(), block_table.data_ptr(),
-                                      block_table.stride(0), block_table.shape[1], n_rows, out.seq_len.data_ptr(),
-                                      out.cu_new.data_ptr(), out.slot_map.data_ptr(), out.positions.data_ptr(),
-                                      out.n_free.data_ptr(), _stream_handle(device))
+    status = _call(lib().gqa_paged_plan, device, cached.data_ptr(), n_new.data_ptr(), batch, free_blocks.data_ptr(),
+                   n_free.data_ptr(), free_blocks.numel(), block_table.data_ptr(), block_table.stride(0),
+                   block_table.shape[1], n_rows, *[t.data_ptr() for t in out])
     check(status, "gqa_paged_plan")
     return out
 
 
 def _q8_layout(pool: Q8Pool, device, max_blocks: int = 1) -> GqaQ8Kv:
     k, v, ks, vs = pool
-    if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype:
+    shape, strides, dtype = k.shape, k.stride(), k.dtype
+    if len(shape) != 4 or v.shape != shape or v.stride() != strides or v.dtype != dtype:
         raise ValueError("k and v of a pool must share dtype, shape [n_blocks,8,16,128] and strides")
-    if k.dtype not in Q8_FORMATS:
+    fmt = Q8_FORMATS.get(dtype)
+    if fmt is None:
         raise ValueError("an 8-bit pool is int8 or float8_e4m3fn")
-    if k.shape[1:] != (N_KV_HEADS, BLOCK_SIZE, HEAD_DIM):
+    n_blocks, heads, rows, dims = shape
+    if heads != N_KV_HEADS or rows != BLOCK_SIZE or dims != HEAD_DIM:
         raise ValueError(f"pools hold {N_KV_HEADS} KV heads of {BLOCK_SIZE} rows of {HEAD_DIM} dimensions per block")
-    if k.stride(3) != 1:
+    if strides[3] != 1:
         raise ValueError("pool rows must be contiguous in head_dim")
-    if ks.shape != k.shape[:2] or vs.shape != ks.shape or ks.stride() != vs.stride() \
+    scale_strides = ks.stride()
+    if ks.shape != shape[:2] or vs.shape != shape[:2] or vs.stride() != scale_strides \
             or ks.dtype != torch.float32 or vs.dtype != torch.float32:
         raise ValueError("k_scale and v_scale must be float32 [n_blocks, 8] with the same strides")
-    for name, t in zip(Q8Pool._fields, pool):
-        if not t.is_cuda or t.device != device:
-            raise ValueError(f"{name} must be on the GPU, on the other tensors' device")
-    return GqaQ8Kv(k.stride(0), k.stride(1), k.stride(2), ks.stride(0), ks.stride(1), BLOCK_SIZE, max_blocks,
-                   k.shape[0], Q8_FORMATS[k.dtype])
+    if not k.device == v.device == ks.device == vs.device == device:
+        raise ValueError("a pool's tensors must be on the GPU, on the other tensors' device")
+    return GqaQ8Kv(strides[0], strides[1], strides[2], scale_strides[0], scale_strides[1], BLOCK_SIZE, max_blocks,
+                   n_blocks, fmt)
 
 
 def _rows(t: torch.Tensor, name: str, heads: int, align: int, copy: bool = True) -> torch.Tensor:
@@ -145,9 +162,11 @@ def _rows(t: torch.Tensor, name: str, heads: int, align: int, copy: bool = True)
     heads together; copied (or refused) where the kernels cannot take it as it lies."""
     if not isinstance(t, torch.Tensor) or t.dim() != 3 or t.dtype != torch.bfloat16 or not t.is_cuda:
         raise ValueError(f"{name} must be a bfloat16 [N, {heads}, 128] tensor on the GPU")
-    if t.shape[1:] != (heads, HEAD_DIM):
-        raise _lib.GqaConfigError(_lib.GQA_ERR_INVALID_CONFIG, f"{name} of {t.shape[1]} heads of {t.shape[2]}")
-    if t.stride(2) != 1 or t.stride(1) != HEAD_DIM or t.stride(0) < 0 or t.stride(0) * 2 % align or t.data_ptr() % align:
+    n, h, d = t.shape
+    if h != heads or d != HEAD_DIM:
+        raise _lib.GqaConfigError(_lib.GQA_ERR_INVALID_CONFIG, f"{name} of {h} heads of {d}")
+    token, head, dim = t.stride()
+    if dim != 1 or head != HEAD_DIM or token < 0 or (2 * token | t.data_ptr()) % align:
         if not copy:
             raise ValueError(f"{name}: each token's heads must lie together, tokens {align} bytes aligned")
         t = t.clone(memory_format=torch.contiguous_format)
@@ -175,17 +194,30 @@ def kv_append_q8(k_new: torch.Tensor, v_new: torch.Tensor, pool: Q8Pool, slot_ma
     elif rope_k:
         raise ValueError("rope_k needs positions")
     p = make_params(rope_q=False, rope_k=rope_k, theta=theta)
-    with torch.cuda.device(device):
-        status = lib().gqa_kv_append_q8(ctypes.byref(p), k_new.data_ptr(), k_new.stride(0), v_new.data_ptr(),
-                                        v_new.stride(0), *(t.data_ptr() for t in pool), ctypes.byref(layout),
-                                        slot_map.data_ptr(), None if positions is None else positions.data_ptr(), n,
-                                        _stream_handle(device))
+    status = _call(lib().gqa_kv_append_q8, device, ctypes.byref(p), k_new.data_ptr(), k_new.stride(0),
+                   v_new.data_ptr(), v_new.stride(0), *[t.data_ptr() for t in pool], ctypes.byref(layout),
+                   slot_map.data_ptr(), None if positions is None else positions.data_ptr(), n)
     check(status, "gqa_kv_append_q8")
 
 
 def attention_q8_workspace_bytes(batch: int, n_tokens: int, max_new: int, params: Optional[GqaParams] = None) -> int:
     p = params or make_params()
     return int(lib().gqa_attention_q8_workspace_bytes(ctypes.byref(p), int(batch), int(n_tokens), int(max_new)))
+
+
+def new_attention_q8_workspace(batch: int, n_tokens: int, max_new: int, device="cuda",
+                               params: Optional[GqaParams] = None) -> torch.Tensor:
+    """A workspace for gqa_attention_q8 calls of at most these sizes, its counters cleared on the
+    current stream.  Calls that share it must be ordered (one stream)."""
+    device = torch.empty(0, device=device).device              # ("cuda": the current one)
+    with torch.cuda.device(device):
+        nbytes = attention_q8_workspace_bytes(batch, n_tokens, max_new, params)
+    if nbytes == 0:
+        check(_lib.GQA_ERR_INVALID_CONFIG, "gqa_attention_q8_workspace_bytes")
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    check(_call(lib().gqa_attention_q8_workspace_init, device, workspace.data_ptr(), nbytes),
+          "gqa_attention_q8_workspace_init")
+    return workspace
 
 
 class PreparedAttentionQ8:
@@ -212,13 +244,13 @@ class PreparedAttentionQ8:
             raise ValueError(f"without cu_new q has one row per sequence: {n} rows for {batch} sequences")
         max_new = (n if cu_new is not None else 1) if max_new is None else int(max_new)
         p = params or make_params(rope_q=rope_q, rope_k=False, theta=theta, scale=scale)
+        if workspace is None:
+            workspace = new_attention_q8_workspace(batch, n, max_new, device, p)
         with torch.cuda.device(device):
             nbytes = attention_q8_workspace_bytes(batch, n, max_new, p)
         if nbytes == 0:
             check(_lib.GQA_ERR_INVALID_CONFIG, "gqa_attention_q8_workspace_bytes")
-        if workspace is None:
-            workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        elif workspace.device != device or not workspace.is_contiguous() \
+        if workspace.device != device or not workspace.is_contiguous() \
                 or workspace.numel() * workspace.element_size() < nbytes:
             raise ValueError(f"workspace must be contiguous, on {device}, of {nbytes} bytes at least")
         if out is None:
@@ -234,11 +266,7 @@ class PreparedAttentionQ8:
         self._fn = lib().gqa_attention_q8
 
     def __call__(self) -> torch.Tensor:
-        if torch.cuda.current_device() == self.device.index:
-            status = self._fn(*self._args, _stream_handle(self.device))
-        else:
-            with torch.cuda.device(self.device):
-                status = self._fn(*self._args, _stream_handle(self.device))
+        status = _call(self._fn, self.device, *self._args)
         if status:
             check(status, "gqa_attention_q8")
         return self.out
@@ -257,7 +285,8 @@ def gqa_attention_q8(q: torch.Tensor, pool: Q8Pool, block_table: torch.Tensor, s
                  (None: one row each)
     max_new      a bound on a sequence's rows (a host value; default: N).  Up to 16 rows take the
                  streamed kernel; a tight bound keeps idle launches out
-    workspace    attention_q8_workspace_bytes(B, N, max_new) bytes; calls that share it must be ordered
+    workspace    from new_attention_q8_workspace, for calls up to its sizes (else one is made for the call);
+                 calls that share it must be ordered
     Returns out [N, 32, 128]; rows behind cu_new[B] are left as they were in `out`."""
     q = _rows(q, "q", N_Q_HEADS, 16)
     if isinstance(block_table, torch.Tensor):

@@ -334,7 +334,10 @@ int gqa_kv_append_q8(const gqa_params_t* params, const uint16_t* k_new, int64_t 
  *          aligned); n_tokens rows
  *   out    [n_tokens][32][128]; rows that belong to no sequence are left as they were
  *   max_new  at least every sequence's rows (a host bound; it chooses the kernels)
- *   workspace  gqa_attention_q8_workspace_bytes bytes, 256-byte aligned, any contents
+ *   workspace  gqa_attention_q8_workspace_bytes bytes, 256-byte aligned, cleared once by
+ *          gqa_attention_q8_workspace_init before its first call (its counters read zero between
+ *          calls); then for any calls it is large enough for, one after the other
+ *   batch  at most 32768
  * A sequence of up to 16 rows is streamed: the keys of all (sequence, KV head) pairs are cut into
  * equal ranges; longer ones go in tiles of 64 rows.  A sequence with seq_len[b] below its rows or
  * above 16 * max_blocks, or more than max_new rows, gets NaN rows; where cu_new is not
@@ -343,6 +346,7 @@ int gqa_kv_append_q8(const gqa_params_t* params, const uint16_t* k_new, int64_t 
  * holds behind seq_len[b], or in keys a row does not see, does not reach it.  Arithmetic: fp16
  * products of exact codes with Q and weights of 11 bits, fp32 sums, one BF16 rounding. */
 size_t gqa_attention_q8_workspace_bytes(const gqa_params_t* params, int32_t batch, int32_t n_tokens, int32_t max_new);
+int gqa_attention_q8_workspace_init(void* workspace, size_t workspace_bytes, void* stream);
 int gqa_attention_q8(const gqa_params_t* params, const uint16_t* q, int64_t q_token_stride, const void* k_pool,
                      const void* v_pool, const float* k_scale, const float* v_scale, const gqa_q8_kv_t* kv,
                      const int32_t* block_table, const int32_t* seq_len, const int32_t* cu_new, int32_t batch,

@@ -421,7 +421,7 @@ def test_attention_strides_and_default_arguments(dev):
     fused[:, :32] = q.to(dev)
     wide = [t.view(torch.uint8).permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3).view(t.dtype) for t in p[:2]]
     scales = [t.t().contiguous().t() for t in p[2:]]
-    ws = torch.full((gqa.attention_q8_workspace_bytes(3, 3, 1),), 255, dtype=torch.uint8, device=dev)
+    ws = gqa.new_attention_q8_workspace(3, 3, 1, dev)
     out = torch.empty((3, 32, 128), dtype=torch.bfloat16, device=dev)
     got = gqa.gqa_attention_q8(fused[:, :32], gqa.Q8Pool(*wide, *scales), i32(table, dev), i32([50, 18, 77], dev),
                                workspace=ws, out=out)
