@@ -345,18 +345,18 @@ __device__ __forceinline__ void q8_references(f32x4_t (&s)[kTiles][2], float (&f
 template <int kTiles>
 __device__ __forceinline__ q8_f16x8 q8_weights(const f32x4_t (&s)[2], float f, float lsv, int c, Q8State<kTiles>& st) {
     // (a V scale 2^100 below the column's others': its weights are 0 in fp16 either way)
-    const float base = fminf(st.mv[c] - lsv, st.m[c] + 100.0f);
+    const float base = __builtin_amdgcn_fmed3f(st.mv[c] - lsv, -__builtin_inff(), st.m[c] + 100.0f);
+    float w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j >> 2][j & 3], f, -base));
     q8_f16x8 p;
-    float sum = 0.0f;
 #pragma unroll
     for (int j = 0; j < 8; j += 2) {
-        const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j >> 2][j & 3], f, -base));
-        const float w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j >> 2][(j & 3) + 1], f, -base));
-        const q8_f16x2 w = q8_pack(w0, w1);
-        p[j] = w.x;
-        p[j + 1] = w.y;
-        sum += w0 + w1;
+        const q8_f16x2 two = q8_pack(w[j], w[j + 1]);
+        p[j] = two.x;
+        p[j + 1] = two.y;
     }
+    const float sum = ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
     st.l[c] = __builtin_fmaf(sum, __builtin_amdgcn_exp2f(base - st.m[c]), st.l[c]);
     return p;
 }
@@ -384,24 +384,25 @@ struct Q8Batch {
 };
 typedef GQA_LDS Q8Batch q8_batch;
 
-// The ids of batch n of the sequence with table row `table` and n_blk blocks (past the last: its id).
-__device__ __forceinline__ void request_ids(q8_batch* bt, const int32_t* table, int n, int n_blk, int lane) {
-    copy4(table + min(kWave * n + lane, n_blk - 1), (q8_lds*)bt->id);
+// The ids of steps `step` .. `step` + 31 of the sequence with table row `table` and n_blk blocks (past the
+// last: its id).
+__device__ __forceinline__ void request_ids(q8_batch* bt, const int32_t* table, int step, int n_blk, int lane) {
+    copy4(table + min(2 * step + lane, n_blk - 1), (q8_lds*)bt->id);
 }
 
-// The scales of a batch whose ids have landed.  An id outside the pool becomes block 0 with a NaN scale:
-// the rows that attend to it are NaN.
+// The scales of a batch whose ids have landed.  An id outside the pool stands for block 0 with a NaN
+// scale: the rows that attend to it are NaN.
 __device__ __forceinline__ void request_scales(q8_batch* bt, const Q8Pool& pool, int h, int lane) {
     const int32_t id = bt->id[lane];
     const bool ok = id >= 0 && id < pool.n_blocks;
-    if (!ok) bt->id[lane] = 0;
     const int64_t at = id * pool.scale_block_stride + h * pool.scale_head_stride;
     copy4(ok ? pool.k_scale + at : &kNoScale, (q8_lds*)bt->sk);
     copy4(ok ? pool.v_scale + at : &kNoScale, (q8_lds*)bt->sv);
 }
 
-__device__ __forceinline__ int64_t batch_block(const q8_batch* bt, int step, int which) {
-    return __builtin_amdgcn_readfirstlane(bt->id[2 * (step & 31) + which]);
+__device__ __forceinline__ int64_t batch_block(const q8_batch* bt, const Q8Pool& pool, int step, int which) {
+    const int id = __builtin_amdgcn_readfirstlane(bt->id[2 * (step & 31) + which]);
+    return id >= 0 && id < pool.n_blocks ? id : 0;
 }
 
 // K scale and log2 of the V scale of the lane's block (its keys are 8 (lane / 16) .. of the step).  A
@@ -543,9 +544,10 @@ __device__ __forceinline__ void write_partial(const Q8AttnArgs& a, int64_t row0,
     }
 }
 
-// The n partials of a single token's four rows (one KV head) by one wave: lane (c, i) has dims 8i ..
-// 8i + 7 of column c.  kBatch partials are in flight at once.  row_of(i): partial i's first row.
-template <typename RowOf>
+// out = sum_i O_i 2^(M_i - m) / sum_i l_i 2^(m_i - m) over the n partials of a token's four rows (one KV
+// head), by one wave: lane (c, i) has dims 8i .. 8i + 7 of column c.  kBatch partials are in
+// flight at once.  row_of(i): partial i's first row.  kOne: of this launch.
+template <bool kOne, typename RowOf>
 __device__ __forceinline__ void merge_token(const Q8AttnArgs& a, int n, RowOf row_of, uint16_t* out, int lane) {
     constexpr int kBatch = 8;
     const Q8Shared parts(a);
@@ -555,10 +557,16 @@ __device__ __forceinline__ void merge_token(const Q8AttnArgs& a, int n, RowOf ro
         f32x4_t ml[kBatch], x[kBatch][2];
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
-            const int row = row_of(min(i0 + j, n - 1)) + c;
-            ml[j] = Q8Shared::get(parts.ml, row * 16);
-            x[j][0] = Q8Shared::get(parts.rows, (row * kD + i8) * 4);
-            x[j][1] = Q8Shared::get(parts.rows, (row * kD + i8) * 4 + 16);
+            const int64_t row = row_of(min(i0 + j, n - 1)) + c;
+            if constexpr (kOne) {
+                ml[j] = Q8Shared::get(parts.ml, static_cast<int>(row) * 16);
+                x[j][0] = Q8Shared::get(parts.rows, (static_cast<int>(row) * kD + i8) * 4);
+                x[j][1] = Q8Shared::get(parts.rows, (static_cast<int>(row) * kD + i8) * 4 + 16);
+            } else {
+                ml[j] = *reinterpret_cast<const f32x4_t*>(a.part_ml + row);
+                x[j][0] = *reinterpret_cast<const f32x4_t*>(a.part_o + row * kD + i8);
+                x[j][1] = *reinterpret_cast<const f32x4_t*>(a.part_o + row * kD + i8 + 4);
+            }
         }
         float top = m, topv = mv;
 #pragma unroll
@@ -714,7 +722,7 @@ void q8_stream_kernel(Q8AttnArgs a) {
     int since = 0;                                 // steps requested since the last ids were
     auto following = [](int slot) { return slot + 1 == kBatches ? 0 : slot + 1; };
     auto ids = [&](const Piece& p, int n) {
-        request_ids(batches + following(feed_slot), a.block_table + static_cast<int64_t>(p.b) * a.max_blocks, n,
+        request_ids(batches + following(feed_slot), a.block_table + static_cast<int64_t>(p.b) * a.max_blocks, 32 * n,
                     (p.start + p.n - 1) / kQ8Block + 1, lane);
         since = 0;
     };
@@ -739,7 +747,7 @@ void q8_stream_kernel(Q8AttnArgs a) {
             else ids_due = true;
         }
         const q8_batch* bt = batches + feed_slot;
-        const int64_t id0 = batch_block(bt, feed_step, 0), id1 = batch_block(bt, feed_step, 1);
+        const int64_t id0 = batch_block(bt, a.pool, feed_step, 0), id1 = batch_block(bt, a.pool, feed_step, 1);
         q8_lds* dst = ring + feed_buf * 2 * kQ8PlaneB;
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
@@ -854,20 +862,25 @@ void q8_stream_kernel(Q8AttnArgs a) {
         for (; last; last &= last - 1) {
             const Part part = (last & 1) ? entering : leaving;
             auto row_of = [&](int i) {
-                return (2 * ((part.r0 + i) * kHkv + h) + (i == 0 ? 1 : 0)) * kGroup;
+                return (2 * (static_cast<int64_t>(part.r0 + i) * kHkv + h) + (i == 0 ? 1 : 0)) * kGroup;
             };
-            merge_token(a, part.n, row_of, a.out + (static_cast<int64_t>(part.row0) * kHq + kGroup * h) * kD, lane);
+            merge_token<true>(a, part.n, row_of, a.out + (static_cast<int64_t>(part.row0) * kHq + kGroup * h) * kD, lane);
         }
     }
 }
 
 // ---------------------------------------------------------------------------------------------
-// Tile kernel: sequences of more than kQ8StreamMax new tokens, in tiles of 64 tokens (256 columns
-// of one KV head) per workgroup of 4 waves, 16 tokens each.  The four waves share the K and V
-// steps in LDS.  Where the tiles do not fill the workgroups their keys are cut into runs.
-constexpr int kTileWaves = 4;
+// Tile kernel: sequences of more than kQ8StreamMax new tokens, in tiles of 64 tokens (256 columns of one
+// KV head) per workgroup of 8 waves, 8 tokens (two column tiles) each.  The waves share the K and V
+// steps in LDS, two steps (a stage) at a time, in a ring of three stages: a stage is requested two
+// ahead, and one barrier a stage says both that it has landed and that the oldest is free.  Two
+// waves share a SIMD: one's products run under the other's exponentials.  (Four waves of four
+// column tiles convert K and V half as often but have a SIMD each: 480 us against NOW.)  Where the
+// tiles do not fill the workgroups their keys are cut into runs.
+constexpr int kTileWaves = 8;
 constexpr int kTileCols = kQ8TileTokens * kGroup;
-constexpr int kTileMinRun = 16;            // steps of the shortest run
+constexpr int kTileRing = 3;               // stages
+constexpr int kTileMinRun = 8;             // steps of the shortest run
 
 namespace {
 
@@ -910,28 +923,34 @@ __device__ void find_tile(const Q8AttnArgs& a, int x, int lane, int& b, int& i) 
 // Runs that each tile's keys are cut into: as many as the workgroups can take at once.
 __device__ __forceinline__ int tile_runs(int tiles, int wgs) { return max(1, wgs / max(1, tiles * kHkv)); }
 
-// Of a tile of `steps` steps: steps of a run and how many runs hold any.
+// Steps of a run of a tile of `steps` steps.
 __device__ __forceinline__ int run_steps(int steps, int runs) { return max(kTileMinRun, (steps + runs - 1) / runs); }
+
+__device__ __forceinline__ void tile_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 }  // namespace
 
 template <int kFmt>
-__global__ __launch_bounds__(kTileWaves * kWave) void q8_tile_kernel(Q8AttnArgs a) {
-    constexpr int kTiles = 4;
-    __shared__ __align__(4096) uint8_t s_ring[2][2][kQ8PlaneB];
-    __shared__ Q8Batch s_batch[kTileWaves][2];     // (a copy for each wave: no barrier for them)
+__global__ __launch_bounds__(kTileWaves * kWave) __attribute__((amdgpu_waves_per_eu(2))) void q8_tile_kernel(Q8AttnArgs a) {
+    constexpr int kTiles = 2;
+    constexpr int kTokens = 4 * kTiles;            // of a wave
+    __shared__ __align__(4096) uint8_t s_ring[kTileRing][2][2][kQ8PlaneB];     // [stage][step][K, V]
+    __shared__ Q8Batch s_batch[2];
     __shared__ float2 s_cs[kQ8TileTokens * kPairs];
     const int lane = threadIdx.x & (kWave - 1);
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    q8_lds* const ring = (q8_lds*)&s_ring[0][0][0];
+    q8_lds* const ring = (q8_lds*)&s_ring[0][0][0][0];
+    q8_batch* const batches = (q8_batch*)&s_batch[0];
     const int tiles = count_tiles(a, lane);
     const int runs = tile_runs(tiles, a.tile_wgs);
-    uint32_t kcopy, vcopy;
+    // Of each step wave w copies rows 8 (w % 4) .. + 7, waves 0 .. 3 of K, the others of V.
+    const int part = wv & 3;
+    const bool of_v = wv >= 4;
+    uint32_t copy;
     {
-        const int row = copy_row(wv, lane);
-        const uint32_t at = static_cast<uint32_t>((row & 15) * a.pool.pos_stride);
-        kcopy = at + 16u * ((lane & 7) ^ k_swizzle(row));
-        vcopy = at + 16u * ((lane & 7) ^ v_swizzle(row));
+        const int row = copy_row(part, lane);
+        copy = static_cast<uint32_t>((row & 15) * a.pool.pos_stride) +
+               16u * ((lane & 7) ^ (of_v ? v_swizzle(row) : k_swizzle(row)));
     }
     const uint32_t koff = k_offset(lane), voff = v_offset(lane);
     const int64_t items = static_cast<int64_t>(tiles) * kHkv * runs;
@@ -955,117 +974,122 @@ __global__ __launch_bounds__(kTileWaves * kWave) void q8_tile_kernel(Q8AttnArgs 
         if (first >= end) continue;
         const int n_blk = last / kQ8Block + 1;
         const int32_t* table = a.block_table + static_cast<int64_t>(b) * a.max_blocks;
-        q8_batch* const batches = (q8_batch*)&s_batch[wv][0];
-        const uint8_t* kh = a.pool.k + h * a.pool.head_stride;
-        const uint8_t* vh = a.pool.v + h * a.pool.head_stride;
-        auto request = [&](int step) {
-            if ((step & 31) == 0 && step != first) {
-                wait_copies<0>();
-                request_scales(batches + ((step >> 5) & 1), a.pool, h, lane);
-                request_ids(batches + (~(step >> 5) & 1), table, (step >> 5) + 1, n_blk, lane);
+        const uint8_t* pool = of_v ? a.pool.v + h * a.pool.head_stride : a.pool.k + h * a.pool.head_stride;
+        // Requests the stage of steps first + i and first + i + 1 (a step past the end reads the last block
+        // again; it is not used).  Batch n is steps first + 32 n on; wave 0 brings it, its ids a batch
+        // ahead, its scales with its first stage.
+        auto request = [&](int i, int stage) {
+            q8_batch* bt = batches + ((i >> 5) & 1);
+            if (wv == 0 && (i & 31) == 0) {
+                request_scales(bt, a.pool, h, lane);
+                request_ids(batches + (~(i >> 5) & 1), table, first + i + 32, n_blk, lane);
             }
-            const int64_t at = batch_block(batches + ((step >> 5) & 1), step, wv >> 1) * a.pool.block_stride;
-            q8_lds* dst = ring + (step & 1) * 2 * kQ8PlaneB + wv * 1024;
-            copy16<false>(kh + at, kcopy, dst);
-            copy16<false>(vh + at, vcopy, dst + kQ8PlaneB);
+            q8_lds* dst = ring + (stage * 4 + (of_v ? 1 : 0)) * kQ8PlaneB + part * 1024;
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                copy16<false>(pool + batch_block(bt, a.pool, i + e, part >> 1) * a.pool.block_stride, copy,
+                              dst + e * 2 * kQ8PlaneB);
         };
-        request_ids(batches + ((first >> 5) & 1), table, first >> 5, n_blk, lane);
-        __syncthreads();                           // (the item before is done with the ring and the angles)
+        tile_barrier();                            // (the item before is done with the ring and the angles)
+        if (wv == 0) request_ids(batches, table, first, n_blk, lane);
         fill_angles(a, sq.start + tok0, tokens, s_cs, threadIdx.x, kTileWaves * kWave);
         wait_copies<0>();
-        request_scales(batches + ((first >> 5) & 1), a.pool, h, lane);
-        request_ids(batches + (~(first >> 5) & 1), table, (first >> 5) + 1, n_blk, lane);
-        request(first);
-        __syncthreads();
+        tile_barrier();
+        request(0, 0);
+        if (first + 2 < end) request(2, 1);
         Q8State<kTiles> st;
         q8_f16x8 qop[kTiles][4];
         float qs[kTiles];
         int lim[kTiles];
 #pragma unroll
         for (int c = 0; c < kTiles; ++c) {
-            const int col = 16 * c + (lane & 15), tok = min(16 * wv + (col >> 2), tokens - 1);
+            const int col = 16 * c + (lane & 15), tok = min(kTokens * wv + (col >> 2), tokens - 1);
             const Q8Row raw = fetch_q(q_row(a, sq.row0 + tok0 + tok, h, col & 3), lane >> 4);
             qs[c] = make_q(a, raw, s_cs + tok * kPairs, lane >> 4, qop[c]);
             lim[c] = sq.start + tok0 + tok;
         }
         st.clear();
-        for (int step = first; step < end; ++step) {
-            wait_copies<0>();
-            __syncthreads();                       // the step has landed, and the other buffer is free
-            if (step + 1 < end) request(step + 1);
-            float sk, lsv;
-            batch_scales(batches + ((step >> 5) & 1), step, lane, sk, lsv);
-            const int key0 = step * kQ8Step;
-            const bool masked = key0 + kQ8Step - 1 > sq.start + tok0;
-            q8_lds* kp = ring + (step & 1) * 2 * kQ8PlaneB;
-            if (masked) mask_values<kFmt, kTiles>(kp + kQ8PlaneB, key0, last, lim, threadIdx.x, kTileWaves * kWave, st);
-            f32x4_t s[kTiles][2];
-            float f[kTiles];
-            const Q8KRows k = read_keys(kp, koff);
-            const Q8VRows v = read_values(kp + kQ8PlaneB, voff);
-            __builtin_amdgcn_sched_barrier(0);
-            q8_scores<kFmt, kTiles>(k, qop, s);
-            q8_references<kTiles>(s, f, key0, masked, sk, lsv, qs, lim, lane, st);
-            q8_f16x8 p[kTiles];
+        int stage = 0;
+        for (int step0 = first; step0 < end; step0 += 2) {
+            // This stage has landed (the next one's two copies may be in flight), and every wave is done
+            // with the one before it.
+            if (step0 + 2 < end) wait_copies<2>();
+            else wait_copies<0>();
+            tile_barrier();
+            if (step0 + 4 < end) request(step0 + 4 - first, stage == 0 ? 2 : stage - 1);
 #pragma unroll
-            for (int c = 0; c < kTiles; ++c) p[c] = q8_weights<kTiles>(s[c], f[c], lsv, c, st);
-            q8_values<kFmt, kTiles>(v, p, st);
+            for (int e = 0; e < 2; ++e) {
+                const int step = step0 + e;
+                if (step >= end) break;
+                q8_lds* kp = ring + (stage * 4 + e * 2) * kQ8PlaneB;
+                const int key0 = step * kQ8Step;
+                const bool masked = key0 + kQ8Step - 1 > sq.start + tok0;
+                if (masked)
+                    mask_values<kFmt, kTiles>(kp + kQ8PlaneB, key0, last, lim, threadIdx.x, kTileWaves * kWave, st);
+                const Q8KRows k = read_keys(kp, koff);
+                float sk, lsv;
+                batch_scales(batches + (((step - first) >> 5) & 1), step - first, lane, sk, lsv);
+                const Q8VRows v = read_values(kp + kQ8PlaneB, voff);
+                f32x4_t s[kTiles][2];
+                float f[kTiles];
+                q8_scores<kFmt, kTiles>(k, qop, s);
+                q8_references<kTiles>(s, f, key0, masked, sk, lsv, qs, lim, lane, st);
+                q8_f16x8 p[kTiles];
+#pragma unroll
+                for (int c = 0; c < kTiles; ++c) p[c] = q8_weights<kTiles>(s[c], f[c], lsv, c, st);
+                q8_values<kFmt, kTiles>(v, p, st);
+            }
+            stage = stage + 1 == kTileRing ? 0 : stage + 1;
         }
-        wait_copies<0>();
+        wait_copies<0>();                          // (ids requested past the end)
         if (per >= steps) {
-            write_out<kTiles>(a, sq, tok0 + 16 * wv, h, lane, st);
+            write_out<kTiles>(a, sq, tok0 + kTokens * wv, h, lane, st);
         } else {
             const int64_t slot = (static_cast<int64_t>(tile) * kHkv + h) * runs + run;
-            write_partial<kTiles, false>(a, a.tile_slot0 + slot * kTileCols + 64 * wv, tokens - 16 * wv, lane, st);
+            write_partial<kTiles, false>(a, a.tile_slot0 + slot * kTileCols + 16 * kTiles * wv, tokens - kTokens * wv, lane, st);
         }
     }
 }
 
 // ---------------------------------------------------------------------------------------------
-// Merge kernels: out = sum_i O_i 2^(M_i - m) / sum_i l_i 2^(m_i - m) over the partials of a row, and NaN
-// rows for sequences whose lengths break the rules.
-namespace {
+// Merge kernel: a wave for each of the tokens of (sequence, KV head) in the stream, up to 16, the first
+// `stream` workgroups; then kTileMergeWaves for each (tile, KV head), its tokens in turn.  A KV head's
+// waves run on one XCD, the one whose waves wrote its partials (its L2 may still hold them).
+constexpr int kTileMergeWaves = 16;
 
-// One row by one wave: lane has dims 2 lane, 2 lane + 1.  Partials at row0 + i * stride.
-__device__ __forceinline__ void merge_row(const Q8AttnArgs& a, int64_t row0, int64_t first, int64_t stride, int n, uint16_t* out,
-                                          int lane) {
-    float m = kLowest, mv = kLowest;
-    for (int i = lane; i < n; i += kWave) {
-        const float4 p = a.part_ml[i == 0 ? first : row0 + (i - 1) * stride];
-        m = fmaxf(m, p.x);
-        mv = fmaxf(mv, p.y);
-    }
-    m = wave_max(m);
-    mv = wave_max(mv);
-    float l = 0.0f, x = 0.0f, y = 0.0f;
-#pragma unroll 8
-    for (int i = 0; i < n; ++i) {
-        const int64_t r = i == 0 ? first : row0 + (i - 1) * stride;
-        const float4 p = a.part_ml[r];
-        const float2 o = *reinterpret_cast<const float2*>(a.part_o + r * kD + 2 * lane);
-        const float f = __builtin_amdgcn_exp2f(p.y - mv);
-        l += p.z * __builtin_amdgcn_exp2f(p.x - m);
-        x += o.x * f;
-        y += o.y * f;
-    }
-    const float f = __builtin_amdgcn_exp2f(mv - m) / l;
-    *reinterpret_cast<uint32_t*>(out + 2 * lane) = bf16_pair(x * f, y * f);
-}
-
-}  // namespace
-
-// Grid: (sequence, KV head), groups of 4 columns (one token's).  A wave takes one column.
-__global__ __launch_bounds__(kGroup * kWave) void q8_stream_merge_kernel(Q8AttnArgs a, int cols) {
-    const int lane = threadIdx.x & (kWave - 1), head = threadIdx.x >> 6;
-    const int b = blockIdx.x / kHkv, h = blockIdx.x % kHkv;
-    Q8Seq sq;
-    if (!q8_seq(a, b, sq)) {
-        if (head == 0) write_nan(a, sq, h, lane, blockIdx.y, gridDim.y);
+__global__ __launch_bounds__(kWave) void q8_merge_kernel(Q8AttnArgs a, int cols, int stream, int toks) {
+    const int lane = threadIdx.x;
+    const int h = blockIdx.x % kHkv;
+    auto out_of = [&](int row) { return a.out + (static_cast<int64_t>(row) * kHq + kGroup * h) * kD; };
+    if (static_cast<int>(blockIdx.x) >= stream) {
+        const int tiles = count_tiles(a, lane);
+        const int runs = tile_runs(tiles, a.tile_wgs);
+        const int unit = (blockIdx.x - stream) / kHkv, tile = unit / kTileMergeWaves;
+        if (runs == 1 || tile >= tiles) return;
+        int b, i;
+        find_tile(a, tile, lane, b, i);
+        Q8Seq sq;
+        q8_seq(a, b, sq);
+        const int tokens = min(kQ8TileTokens, sq.n - i * kQ8TileTokens);
+        const int steps = (sq.start + i * kQ8TileTokens + tokens - 1) / kQ8Step + 1;
+        const int per = run_steps(steps, runs);
+        if (per >= steps) return;
+        for (int tok = unit % kTileMergeWaves; tok < tokens; tok += kTileMergeWaves) {
+            auto row_of = [&](int r) {
+                return a.tile_slot0 + ((static_cast<int64_t>(tile) * kHkv + h) * runs + r) * kTileCols + kGroup * tok;
+            };
+            merge_token<false>(a, (steps + per - 1) / per, row_of, out_of(sq.row0 + i * kQ8TileTokens + tok), lane);
+        }
         return;
     }
-    const int tok = blockIdx.y;
+    const int tok = blockIdx.x / kHkv % toks, b = blockIdx.x / kHkv / toks;
+    Q8Seq sq;
+    if (!q8_seq(a, b, sq)) {
+        write_nan(a, sq, h, lane, tok, toks);
+        return;
+    }
     if (sq.n > kQ8StreamMax || tok >= sq.n) return;
-    // The segment's place in the stream.
+    // The sequence's place in the stream.
     int64_t before = 0, all = 0;
     int steps = 0, seqs = 0, seqs_before = 0;
     Q8Window win;
@@ -1086,32 +1110,8 @@ __global__ __launch_bounds__(kGroup * kWave) void q8_stream_merge_kernel(Q8AttnA
     const int64_t x = before + static_cast<int64_t>(cut.lead) * (seqs_before + 1);
     const int64_t r0 = cut.first_range(x), r1 = cut.last_range(x, steps);
     if (r0 == r1) return;                          // one piece: written already
-    const int col = kGroup * tok + head;
-    merge_row(a, 2 * ((r0 + 1) * kHkv + h) * cols + col, (2 * (r0 * kHkv + h) + 1) * cols + col, 2 * kHkv * cols,
-              static_cast<int>(r1 - r0 + 1), a.out + (static_cast<int64_t>(sq.row0 + tok) * kHq + kGroup * h + head) * kD, lane);
-}
-
-// Grid: workgroups of the tile kernel, tokens of a tile.
-__global__ __launch_bounds__(kGroup * kWave) void q8_tile_merge_kernel(Q8AttnArgs a) {
-    const int lane = threadIdx.x & (kWave - 1), head = threadIdx.x >> 6;
-    const int tiles = count_tiles(a, lane);
-    const int runs = tile_runs(tiles, a.tile_wgs);
-    const int at = blockIdx.x;
-    if (runs == 1 || at >= tiles * kHkv) return;
-    const int tile = at / kHkv, h = at % kHkv, tok = blockIdx.y;
-    int b, i;
-    find_tile(a, tile, lane, b, i);
-    Q8Seq sq;
-    q8_seq(a, b, sq);
-    const int t = i * kQ8TileTokens + tok;
-    if (t >= sq.n) return;
-    const int tokens = min(kQ8TileTokens, sq.n - i * kQ8TileTokens);
-    const int steps = (sq.start + i * kQ8TileTokens + tokens - 1) / kQ8Step + 1;
-    const int per = run_steps(steps, runs);
-    if (per >= steps) return;
-    const int64_t row = a.tile_slot0 + static_cast<int64_t>(at) * runs * kTileCols + kGroup * tok + head;
-    merge_row(a, row + kTileCols, row, kTileCols, (steps + per - 1) / per,
-              a.out + (static_cast<int64_t>(sq.row0 + t) * kHq + kGroup * h + head) * kD, lane);
+    auto row_of = [&](int i) { return (2 * ((r0 + i) * kHkv + h) + (i == 0 ? 1 : 0)) * static_cast<int64_t>(cols) + kGroup * tok; };
+    merge_token<false>(a, static_cast<int>(r1 - r0 + 1), row_of, out_of(sq.row0 + tok), lane);
 }
 
 template <int kFmt, int kTiles, bool kOne = false>
@@ -1133,11 +1133,11 @@ static hipError_t launch_attention(const Q8AttnArgs& a, hipStream_t stream) {
     else if (tiles == 2) launch_stream<kFmt, 2>(a, stream);
     else launch_stream<kFmt, 4>(a, stream);
     const int toks = a.max_new < kQ8StreamMax ? a.max_new : kQ8StreamMax;
-    hipLaunchKernelGGL(q8_stream_merge_kernel, dim3(static_cast<unsigned>(a.batch) * kHkv, static_cast<unsigned>(toks)),
-                       dim3(kGroup * kWave), 0, stream, a, 16 * tiles);
-    if (a.max_new > kQ8StreamMax)
-        hipLaunchKernelGGL(q8_tile_merge_kernel, dim3(static_cast<unsigned>(a.tile_wgs), kQ8TileTokens),
-                           dim3(kGroup * kWave), 0, stream, a);
+    const int of_stream = a.batch * kHkv * toks;
+    // (runs > 1 only where the tiles and heads are at most half of the workgroups)
+    const int of_tiles = a.max_new > kQ8StreamMax ? a.tile_wgs / 2 / kHkv * kHkv * kTileMergeWaves : 0;
+    hipLaunchKernelGGL(q8_merge_kernel, dim3(static_cast<unsigned>(of_stream + of_tiles)), dim3(kWave), 0, stream, a, 16 * tiles,
+                       of_stream, toks);
     return hipGetLastError();
 }
 
