@@ -871,15 +871,21 @@ void q8_stream_kernel(Q8AttnArgs a) {
 
 // ---------------------------------------------------------------------------------------------
 // Tile kernel: sequences of more than kQ8StreamMax new tokens, in tiles of 64 tokens (256 columns of one
-// KV head) per workgroup of 8 waves, 8 tokens (two column tiles) each.  The waves share the K and V
-// steps in LDS, two steps (a stage) at a time, in a ring of three stages: a stage is requested two
-// ahead, and one barrier a stage says both that it has landed and that the oldest is free.  Two
-// waves share a SIMD: one's products run under the other's exponentials.  (Four waves of four
-// column tiles convert K and V half as often but have a SIMD each: 480 us against NOW.)  Where the
-// tiles do not fill the workgroups their keys are cut into runs.
+// KV head) per workgroup of 8 waves, 8 tokens (two column tiles) each.  Two waves share a SIMD: one's
+// products run under the other's exponentials.
+//
+// What bounds it is the issue of vector instructions (the exponentials and what is around them), so
+// the workgroup converts K and V to fp16 once for its eight waves: two steps (a stage) at a time,
+// each thread 16 codes of K and of V, read into registers while the stage before is worked on and
+// written to the other of two fp16 buffers behind it, with one barrier a stage.  (Codes in LDS
+// that every wave converts for itself: 348 us for a chunk of 512 over 8192, 4 sequences; four waves of
+// four column tiles, a SIMD each: 480.)  Where the tiles do not fill the workgroups their keys are
+// cut into runs.
 constexpr int kTileWaves = 8;
 constexpr int kTileCols = kQ8TileTokens * kGroup;
-constexpr int kTileRing = 3;               // stages
+constexpr int kTileKeys = 2 * kQ8Step;     // of a stage
+constexpr int kTileRowB = 2 * kD;          // bytes of a row in fp16
+constexpr int kTilePlaneB = kQ8Step * kTileRowB;       // K (or V) of a step in fp16
 constexpr int kTileMinRun = 8;             // steps of the shortest run
 
 namespace {
@@ -928,31 +934,100 @@ __device__ __forceinline__ int run_steps(int steps, int runs) { return max(kTile
 
 __device__ __forceinline__ void tile_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+typedef short q8_i16x4 __attribute__((ext_vector_type(4)));
+
+// Rows of 256 bytes in 16 chunks of 16.  K: chunk c of row r sits at c ^ k_swizzle(r); V: the 32 bytes
+// of 16 dims, number d, at d ^ (r & 7): the rows that one operand read touches together lie in
+// different banks.
+//
+// This lane's reads: K row as in the 8-bit planes, slice s (8 dims: chunk 2 (g + 4 (s / 2)) + s % 2) by
+// exclusive or; V, transposed: of each 16 lanes, lane r names 8 bytes of row 8g + r / 4 (and of
+// the row 4 on) and gets dim r of the 4 rows.
+__device__ __forceinline__ uint32_t k16_offset(int lane) {
+    const int g = lane >> 4, r = lane & 15, row = 8 * (r >> 2) + (r & 3);
+    return static_cast<uint32_t>(row * kTileRowB + 16 * ((2 * g) ^ k_swizzle(row)));
+}
+
+__device__ __forceinline__ uint32_t v16_offset(int lane) {
+    const int g = lane >> 4, r = lane & 15, row = 8 * g + (r >> 2);
+    return static_cast<uint32_t>(row * kTileRowB + 32 * (row & 7) + 8 * (r & 3));
+}
+
+__device__ __forceinline__ q8_f16x8 read_k16(const q8_lds* kp, uint32_t koff, int t, int s) {
+    return *(const GQA_LDS q8_f16x8*)(kp + (koff ^ (16u * (s & 1) + 128u * (s >> 1))) + 4 * kTileRowB * t);
+}
+
+__device__ __forceinline__ q8_f16x8 read_v16(const q8_lds* vp, uint32_t voff, int dt) {
+    const uint32_t at = voff ^ (32u * dt);
+    struct {
+        q8_i16x4 lo, hi;
+    } two = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((GQA_LDS q8_i16x4*)(vp + at)),
+             __builtin_amdgcn_ds_read_tr16_b64_v4i16((GQA_LDS q8_i16x4*)(vp + (at ^ 128u) + 4 * kTileRowB))};
+    return __builtin_bit_cast(q8_f16x8, two);
+}
+
+// As mask_values, of a V plane in fp16 whose rows behind the sequence's end are zero already: NaNs are
+// marked for the columns that see them and cleared.
+template <int kTiles>
+__device__ __forceinline__ void mask_nan16(q8_lds* vp, int key0, const int (&lim)[kTiles], int tid, Q8State<kTiles>& st) {
+    const int lane = tid & (kWave - 1), g = lane >> 4;
+    bool any = false;
+    for (int i = lane; i < kTilePlaneB / 16; i += kWave) {
+        const q8_f16x8 x = *(const GQA_LDS q8_f16x8*)(vp + 16 * i);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) any |= x[j] != x[j];
+    }
+    if (!__any(any)) return;                       // (the same for every wave: each looked at the whole plane)
+    const uint32_t voff = v16_offset(lane);
+#pragma unroll 1
+    for (int dt = 0; dt < 8; ++dt) {
+        const q8_f16x8 x = read_v16(vp, voff, dt);
+        q8_f16x8 is;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) is[j] = x[j] != x[j] ? (_Float16)1.0f : (_Float16)0.0f;
+#pragma unroll
+        for (int c = 0; c < kTiles; ++c) {
+            q8_f16x8 sees;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sees[j] = key0 + 8 * g + j <= lim[c] ? (_Float16)1.0f : (_Float16)0.0f;
+            const f32x4_t count = __builtin_amdgcn_mfma_f32_16x16x32_f16(is, sees, f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) st.nan[c] |= (count[i] > 0.0f ? 1u : 0u) << (4 * dt + i);
+        }
+    }
+    tile_barrier();
+    for (int i = tid; i < kTilePlaneB / 16; i += kTileWaves * kWave) {
+        GQA_LDS q8_f16x8* at = (GQA_LDS q8_f16x8*)(vp + 16 * i);
+        q8_f16x8 x = *at;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = x[j] != x[j] ? (_Float16)0.0f : x[j];
+        *at = x;
+    }
+    tile_barrier();
+}
+
 }  // namespace
 
 template <int kFmt>
 __global__ __launch_bounds__(kTileWaves * kWave) __attribute__((amdgpu_waves_per_eu(2))) void q8_tile_kernel(Q8AttnArgs a) {
     constexpr int kTiles = 2;
     constexpr int kTokens = 4 * kTiles;            // of a wave
-    __shared__ __align__(4096) uint8_t s_ring[kTileRing][2][2][kQ8PlaneB];     // [stage][step][K, V]
+    __shared__ __align__(4096) uint8_t s_stage[2][2][2][kTilePlaneB];          // [buffer][step][K, V]
     __shared__ Q8Batch s_batch[2];
     __shared__ float2 s_cs[kQ8TileTokens * kPairs];
-    const int lane = threadIdx.x & (kWave - 1);
-    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    q8_lds* const ring = (q8_lds*)&s_ring[0][0][0][0];
+    const int tid = threadIdx.x, lane = tid & (kWave - 1);
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    q8_lds* const stages = (q8_lds*)&s_stage[0][0][0][0];
     q8_batch* const batches = (q8_batch*)&s_batch[0];
     const int tiles = count_tiles(a, lane);
     const int runs = tile_runs(tiles, a.tile_wgs);
-    // Of each step wave w copies rows 8 (w % 4) .. + 7, waves 0 .. 3 of K, the others of V.
-    const int part = wv & 3;
-    const bool of_v = wv >= 4;
-    uint32_t copy;
-    {
-        const int row = copy_row(part, lane);
-        copy = static_cast<uint32_t>((row & 15) * a.pool.pos_stride) +
-               16u * ((lane & 7) ^ (of_v ? v_swizzle(row) : k_swizzle(row)));
-    }
-    const uint32_t koff = k_offset(lane), voff = v_offset(lane);
+    // This thread's part of a stage: 16 codes of row tid / 8, chunk tid % 8.  (A wave's 8 rows lie in one
+    // block, the stage's wv / 2.)
+    const int row = tid >> 3, chunk = tid & 7, row32 = row & 31;
+    const uint32_t src = static_cast<uint32_t>((row & 15) * a.pool.pos_stride + 16 * chunk);
+    const uint32_t kdst = (row >> 5) * 2 * kTilePlaneB + row32 * kTileRowB + 16 * ((2 * chunk) ^ k_swizzle(row32));
+    const uint32_t vdst = (row >> 5) * 2 * kTilePlaneB + kTilePlaneB + row32 * kTileRowB + 32 * (chunk ^ (row32 & 7));
+    const uint32_t koff = k16_offset(lane), voff = v16_offset(lane);
     const int64_t items = static_cast<int64_t>(tiles) * kHkv * runs;
     for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
         const int h = static_cast<int>(item % kHkv);
@@ -974,29 +1049,39 @@ __global__ __launch_bounds__(kTileWaves * kWave) __attribute__((amdgpu_waves_per
         if (first >= end) continue;
         const int n_blk = last / kQ8Block + 1;
         const int32_t* table = a.block_table + static_cast<int64_t>(b) * a.max_blocks;
-        const uint8_t* pool = of_v ? a.pool.v + h * a.pool.head_stride : a.pool.k + h * a.pool.head_stride;
-        // Requests the stage of steps first + i and first + i + 1 (a step past the end reads the last block
+        const uint8_t* kh = a.pool.k + h * a.pool.head_stride;
+        const uint8_t* vh = a.pool.v + h * a.pool.head_stride;
+        // Reads the stage of steps first + i and first + i + 1 (a step past the end reads the last block
         // again; it is not used).  Batch n is steps first + 32 n on; wave 0 brings it, its ids a batch
         // ahead, its scales with its first stage.
-        auto request = [&](int i, int stage) {
+        uint4 rk, rv;
+        auto read = [&](int i) {
             q8_batch* bt = batches + ((i >> 5) & 1);
             if (wv == 0 && (i & 31) == 0) {
                 request_scales(bt, a.pool, h, lane);
                 request_ids(batches + (~(i >> 5) & 1), table, first + i + 32, n_blk, lane);
             }
-            q8_lds* dst = ring + (stage * 4 + (of_v ? 1 : 0)) * kQ8PlaneB + part * 1024;
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-                copy16<false>(pool + batch_block(bt, a.pool, i + e, part >> 1) * a.pool.block_stride, copy,
-                              dst + e * 2 * kQ8PlaneB);
+            const int64_t at = batch_block(bt, a.pool, i + (wv >> 2), (wv >> 1) & 1) * a.pool.block_stride;
+            rk = *reinterpret_cast<const uint4*>(kh + at + src);
+            rv = *reinterpret_cast<const uint4*>(vh + at + src);
         };
-        tile_barrier();                            // (the item before is done with the ring and the angles)
-        if (wv == 0) request_ids(batches, table, first, n_blk, lane);
-        fill_angles(a, sq.start + tok0, tokens, s_cs, threadIdx.x, kTileWaves * kWave);
-        wait_copies<0>();
+        // ... and writes it as fp16, V rows behind the last key as zeros.
+        auto convert = [&](int i) {
+            if ((first + i) * kQ8Step + row > last) rv = make_uint4(0u, 0u, 0u, 0u);
+            q8_lds* dst = stages + ((i >> 1) & 1) * 4 * kTilePlaneB;
+            *(GQA_LDS q8_f16x8*)(dst + kdst) = q8_eight<kFmt>(rk.x, rk.y);
+            *(GQA_LDS q8_f16x8*)(dst + (kdst ^ 16u)) = q8_eight<kFmt>(rk.z, rk.w);
+            *(GQA_LDS q8_f16x8*)(dst + vdst) = q8_eight<kFmt>(rv.x, rv.y);
+            *(GQA_LDS q8_f16x8*)(dst + vdst + 16) = q8_eight<kFmt>(rv.z, rv.w);
+        };
+        tile_barrier();                            // (the item before is done with the buffers and the angles)
+        if (wv == 0) {
+            request_ids(batches, table, first, n_blk, lane);
+            wait_copies<0>();
+        }
+        fill_angles(a, sq.start + tok0, tokens, s_cs, tid, kTileWaves * kWave);
         tile_barrier();
-        request(0, 0);
-        if (first + 2 < end) request(2, 1);
+        read(0);
         Q8State<kTiles> st;
         q8_f16x8 qop[kTiles][4];
         float qs[kTiles];
@@ -1009,39 +1094,58 @@ __global__ __launch_bounds__(kTileWaves * kWave) __attribute__((amdgpu_waves_per
             lim[c] = sq.start + tok0 + tok;
         }
         st.clear();
-        int stage = 0;
+        convert(0);
+        if (wv == 0) wait_copies<0>();             // the first batch's scales
+        tile_barrier();
         for (int step0 = first; step0 < end; step0 += 2) {
-            // This stage has landed (the next one's two copies may be in flight), and every wave is done
-            // with the one before it.
-            if (step0 + 2 < end) wait_copies<2>();
-            else wait_copies<0>();
-            tile_barrier();
-            if (step0 + 4 < end) request(step0 + 4 - first, stage == 0 ? 2 : stage - 1);
+            const bool more = step0 + 2 < end;
+            if (more) read(step0 + 2 - first);
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int step = step0 + e;
                 if (step >= end) break;
-                q8_lds* kp = ring + (stage * 4 + e * 2) * kQ8PlaneB;
+                q8_lds* kp = stages + ((((step0 - first) >> 1) & 1) * 4 + e * 2) * kTilePlaneB;
+                q8_lds* vp = kp + kTilePlaneB;
                 const int key0 = step * kQ8Step;
                 const bool masked = key0 + kQ8Step - 1 > sq.start + tok0;
-                if (masked)
-                    mask_values<kFmt, kTiles>(kp + kQ8PlaneB, key0, last, lim, threadIdx.x, kTileWaves * kWave, st);
-                const Q8KRows k = read_keys(kp, koff);
+                if (kFmt == kQ8E4m3 && masked) mask_nan16<kTiles>(vp, key0, lim, tid, st);
                 float sk, lsv;
                 batch_scales(batches + (((step - first) >> 5) & 1), step - first, lane, sk, lsv);
-                const Q8VRows v = read_values(kp + kQ8PlaneB, voff);
                 f32x4_t s[kTiles][2];
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    q8_f16x8 k[4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) k[q] = read_k16(kp, koff, t, q);
+#pragma unroll
+                    for (int c = 0; c < kTiles; ++c) {
+                        f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[q], qop[c][q], acc, 0, 0, 0);
+                        s[c][t] = acc;
+                    }
+                }
                 float f[kTiles];
-                q8_scores<kFmt, kTiles>(k, qop, s);
                 q8_references<kTiles>(s, f, key0, masked, sk, lsv, qs, lim, lane, st);
                 q8_f16x8 p[kTiles];
 #pragma unroll
                 for (int c = 0; c < kTiles; ++c) p[c] = q8_weights<kTiles>(s[c], f[c], lsv, c, st);
-                q8_values<kFmt, kTiles>(v, p, st);
+                q8_f16x8 v[8];
+#pragma unroll
+                for (int dt = 0; dt < 8; ++dt) v[dt] = read_v16(vp, voff, dt);
+#pragma unroll
+                for (int dt = 0; dt < 8; ++dt)
+#pragma unroll
+                    for (int c = 0; c < kTiles; ++c)
+                        st.o[c][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[dt], p[c], st.o[c][dt], 0, 0, 0);
             }
-            stage = stage + 1 == kTileRing ? 0 : stage + 1;
+            if (more) {
+                convert(step0 + 2 - first);
+                if (wv == 0 && ((step0 + 2 - first) & 31) == 0) wait_copies<0>();      // the batch's scales
+                tile_barrier();
+            }
         }
-        wait_copies<0>();                          // (ids requested past the end)
+        if (wv == 0) wait_copies<0>();             // (ids requested past the end)
         if (per >= steps) {
             write_out<kTiles>(a, sq, tok0 + kTokens * wv, h, lane, st);
         } else {
