@@ -780,22 +780,27 @@ void q8_stream_kernel(Q8AttnArgs a) {
 
     ids(cur, cur.first / 32);
     int slot = 0, buf = 0;
-    Q8State<kTiles> st;
-    while (true) {
-        Q8Row raw[kTiles];
+    // The piece cur, of at most 4 kNow tokens.  The kernel of four column tiles meets many single tokens
+    // (decodes beside prompt chunks) and works on their one tile alone: 87 -> 70 us for 22 decodes and two
+    // chunks of 301 tokens.  (Two tiles stay within the time of the reads: 113 us either way for 64
+    // sequences of 8 tokens over 512..8192.)
+    auto work = [&](auto now) {
+        constexpr int kNow = decltype(now)::value;
+        Q8State<kNow> st;
+        Q8Row raw[kNow];
 #pragma unroll
-        for (int c = 0; c < kTiles; ++c) {
+        for (int c = 0; c < kNow; ++c) {
             const int col = 16 * c + (lane & 15);
             raw[c] = fetch_q(q_row(a, cur.row0 + min(col >> 2, cur.n - 1), h, col & 3), lane >> 4);
         }
         while (ahead < kRing - 1 && request()) {}
         fill_angles(a, cur.start, cur.n, s_cs, lane, kWave);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        q8_f16x8 qop[kTiles][4];
-        float qs[kTiles];
-        int lim[kTiles];
+        q8_f16x8 qop[kNow][4];
+        float qs[kNow];
+        int lim[kNow];
 #pragma unroll
-        for (int c = 0; c < kTiles; ++c) {
+        for (int c = 0; c < kNow; ++c) {
             const int tok = min((16 * c + (lane & 15)) >> 2, cur.n - 1);
             qs[c] = make_q(a, raw[c], s_cs + tok * kPairs, lane >> 4, qop[c]);
             lim[c] = cur.start + tok;
@@ -809,35 +814,39 @@ void q8_stream_kernel(Q8AttnArgs a) {
             buf = buf + 1 == kRing ? 0 : buf + 1;
             const int key0 = step * kQ8Step;
             const bool masked = key0 + kQ8Step - 1 > cur.start;
-            if (masked) mask_values<kFmt, kTiles>(vp, key0, cur.start + cur.n - 1, lim, lane, kWave, st);
+            if (masked) mask_values<kFmt, kNow>(vp, key0, cur.start + cur.n - 1, lim, lane, kWave, st);
             const Q8KRows k = read_keys(kp, koff);
             float sk, lsv;
             batch_scales(batches + slot, step, lane, sk, lsv);
             const Q8VRows v = read_values(vp, voff);
             __builtin_amdgcn_sched_barrier(0);
-            f32x4_t s[kTiles][2];
-            q8_scores<kFmt, kTiles>(k, qop, s);
-            float f[kTiles];
-            q8_references<kTiles>(s, f, key0, masked, sk, lsv, qs, lim, lane, st);
-            q8_f16x8 p[kTiles];
+            f32x4_t s[kNow][2];
+            q8_scores<kFmt, kNow>(k, qop, s);
+            float f[kNow];
+            q8_references<kNow>(s, f, key0, masked, sk, lsv, qs, lim, lane, st);
+            q8_f16x8 p[kNow];
 #pragma unroll
-            for (int c = 0; c < kTiles; ++c) p[c] = q8_weights<kTiles>(s[c], f[c], lsv, c, st);
-            q8_values<kFmt, kTiles>(v, p, st);
+            for (int c = 0; c < kNow; ++c) p[c] = q8_weights<kNow>(s[c], f[c], lsv, c, st);
+            q8_values<kFmt, kNow>(v, p, st);
             if ((step & 31) == 31 || step + 1 == cur.end) slot = following(slot);
             --ahead;
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // the buffer's reads are done before it is refilled
         }
         const Q8Seq sq{cur.row0, cur.n, cur.start};
         if (cur.first == 0 && cur.end == cur.steps) {
-            write_out<kTiles>(a, sq, 0, h, lane, st);
+            write_out<kNow>(a, sq, 0, h, lane, st);
         } else {
             constexpr int kCols = kOne ? kGroup : 16 * kTiles;
-            write_partial<kTiles, kOne>(a, (2 * static_cast<int64_t>(wave) + (cur.first == 0 ? 1 : 0)) * kCols, cur.n, lane, st);
+            write_partial<kNow, kOne>(a, (2 * static_cast<int64_t>(wave) + (cur.first == 0 ? 1 : 0)) * kCols, cur.n, lane, st);
             if constexpr (kOne) {                  // counted when the wave has no more to request
                 const int r0 = cut.first_range(cur.at), n = cut.last_range(cur.at, cur.steps) - r0 + 1;
                 (cur.first == 0 ? leaving : entering) = Part{cur.b, cur.row0, r0, n};
             }
         }
+    };
+    while (true) {
+        if (kTiles == 4 && cur.n <= 4) work(std::integral_constant<int, 1>{});
+        else work(std::integral_constant<int, kTiles>{});
         if (!have_next) break;
         cur = next;                                // (which the last request has entered: feed is `cur` now)
         feed_next = false;
@@ -877,9 +886,11 @@ void q8_stream_kernel(Q8AttnArgs a) {
 // What bounds it is the issue of vector instructions (the exponentials and what is around them), so
 // the workgroup converts K and V to fp16 once for its eight waves: two steps (a stage) at a time,
 // each thread 16 codes of K and of V, read into registers while the stage before is worked on and
-// written to the other of two fp16 buffers behind it, with one barrier a stage.  (Codes in LDS
-// that every wave converts for itself: 348 us for a chunk of 512 over 8192, 4 sequences; four waves of
-// four column tiles, a SIMD each: 480.)  Where the tiles do not fill the workgroups their keys are
+// written to the other of two fp16 buffers behind it, with one barrier a stage.  4 sequences with
+// chunks of 512 tokens over 8192 take 309 us: 920 TFLOP/s of products.  (Codes in LDS that every wave
+// converts for itself: 348 us; only V as codes: 337; four waves of four column tiles, a SIMD each: 480.)
+// What is left is LDS: a wave reads 16 KB a step, its workgroup 128 KB in about 1024 of the step's 1200
+// clocks.  Where the tiles do not fill the workgroups their keys are
 // cut into runs.
 constexpr int kTileWaves = 8;
 constexpr int kTileCols = kQ8TileTokens * kGroup;
@@ -1159,7 +1170,7 @@ __global__ __launch_bounds__(kTileWaves * kWave) __attribute__((amdgpu_waves_per
 // Merge kernel: a wave for each of the tokens of (sequence, KV head) in the stream, up to 16, the first
 // `stream` workgroups; then kTileMergeWaves for each (tile, KV head), its tokens in turn.  A KV head's
 // waves run on one XCD, the one whose waves wrote its partials (its L2 may still hold them).
-constexpr int kTileMergeWaves = 16;
+constexpr int kTileMergeWaves = 32;          // (16: 1.2 us more for two chunks of 301 tokens)
 
 __global__ __launch_bounds__(kWave) void q8_merge_kernel(Q8AttnArgs a, int cols, int stream, int toks) {
     const int lane = threadIdx.x;
