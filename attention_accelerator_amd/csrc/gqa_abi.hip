@@ -3,6 +3,7 @@
 // Validation mirrors the reference core's start-time rejection
 // (gqa_attention_wrapper.v:230-244): a rejected call launches nothing and writes no
 // output, and the status says why.
+#include <algorithm>
 #include <cmath>
 #include <cstdlib>
 #include <cstring>
@@ -763,6 +764,34 @@ bool q8_layout_ok(const gqa_q8_kv_t* kv) {
            (kv->format == GQA_Q8_INT8 || kv->format == GQA_Q8_E4M3);
 }
 
+// Whether no two elements of a pool of these strides lie in the same place (they may for reads alone):
+// each stride passes what lies below it.
+bool q8_distinct(const gqa_q8_kv_t* kv) {
+    struct Dim {
+        int64_t stride, size;
+    };
+    auto distinct = [](Dim* d, int n, int64_t extent) {
+        std::sort(d, d + n, [](const Dim& x, const Dim& y) { return x.stride < y.stride; });
+        for (int i = 0; i < n; ++i) {
+            if (d[i].size == 1) continue;
+            if (d[i].stride < extent) return false;
+            if (__builtin_mul_overflow(d[i].stride, d[i].size - 1, &d[i].stride) ||
+                __builtin_add_overflow(extent, d[i].stride, &extent))
+                return false;
+        }
+        return true;
+    };
+    Dim rows[3] = {{kv->pos_stride, 16}, {kv->head_stride, kHkv}, {kv->block_stride, kv->n_blocks}};
+    Dim scales[2] = {{kv->scale_head_stride, kHkv}, {kv->scale_block_stride, kv->n_blocks}};
+    return distinct(rows, 3, kD) && distinct(scales, 2, 1);
+}
+
+// Whether [p, p + bytes) and [q, q + more) meet.
+bool overlap(const void* p, int64_t bytes, const void* q, int64_t more) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(p), y = reinterpret_cast<uintptr_t>(q);
+    return p && q && bytes > 0 && more > 0 && x < y + more && y < x + bytes;
+}
+
 bool q8_pool_aligned(const gqa_q8_kv_t* kv, const void* k, const void* v, const void* ks, const void* vs) {
     return aligned(k, 16) && aligned(v, 16) && aligned(ks, 4) && aligned(vs, 4) && kv->pos_stride % 16 == 0 &&
            kv->head_stride % 16 == 0 && kv->block_stride % 16 == 0;
@@ -827,11 +856,17 @@ int gqa_paged_plan(const int32_t* cached, const int32_t* n_new, int32_t batch, c
                           static_cast<const void*>(cu_new), static_cast<const void*>(slot_map),
                           static_cast<const void*>(positions), static_cast<const void*>(n_free_out)})
         if (!aligned(p, 4)) return GQA_ERR_BAD_POINTER;
-    // Workgroups read the lengths while others write: an output that starts at an input races.
-    for (const void* p : {static_cast<const void*>(seq_len), static_cast<const void*>(cu_new),
-                          static_cast<const void*>(slot_map), static_cast<const void*>(positions),
-                          static_cast<const void*>(n_free_out)})
-        if (p && (p == cached || p == n_new || p == free_blocks || p == n_free)) return GQA_ERR_BAD_POINTER;
+    // Workgroups read the inputs while others write: no output may meet an input or another output.
+    const struct {
+        const void* p;
+        int64_t n;
+    } arrays[] = {{cached, batch},       {n_new, batch},      {free_blocks, free_capacity}, {n_free, 1},
+                  {block_table, (batch - 1) * table_stride + max_blocks},
+                  {seq_len, batch},      {cu_new, int64_t{batch} + 1}, {slot_map, n_rows},  {positions, n_rows},
+                  {n_free_out, 1}};
+    for (int i = 4; i < 10; ++i)
+        for (int j = 0; j < i; ++j)
+            if (overlap(arrays[i].p, 4 * arrays[i].n, arrays[j].p, 4 * arrays[j].n)) return GQA_ERR_BAD_POINTER;
     PagedPlanArgs a{};
     a.cached = cached;
     a.n_new = n_new;
@@ -863,8 +898,10 @@ int gqa_kv_append_q8(const gqa_params_t* params, const uint16_t* k_new, int64_t 
     if (!k_new || !v_new || !k_pool || !v_pool || !k_scale || !v_scale || !slots || (rope && !positions))
         return GQA_ERR_BAD_POINTER;
     if (!aligned(k_new, 8) || !aligned(v_new, 8) || k_token_stride % 4 || v_token_stride % 4 || !aligned(slots, 4) ||
-        !aligned(positions, 4) || !q8_pool_aligned(kv, k_pool, v_pool, k_scale, v_scale))
+        !aligned(positions, 4) || !q8_pool_aligned(kv, k_pool, v_pool, k_scale, v_scale) || k_pool == v_pool ||
+        k_scale == v_scale)
         return GQA_ERR_BAD_POINTER;
+    if (!q8_distinct(kv)) return GQA_ERR_INVALID_CONFIG;
     Q8AppendArgs a{};
     a.pool = q8_pool(kv, k_pool, v_pool, k_scale, v_scale);
     a.k_new = k_new;
@@ -907,6 +944,8 @@ int gqa_attention_q8(const gqa_params_t* params, const uint16_t* q, int64_t q_to
     if (!aligned(q, 16) || q_token_stride % 8 || !aligned(out, 8) || !aligned(block_table, 4) || !aligned(seq_len, 4) ||
         !aligned(cu_new, 4) || !q8_pool_aligned(kv, k_pool, v_pool, k_scale, v_scale))
         return GQA_ERR_BAD_POINTER;
+    constexpr int64_t kRow = int64_t{kHq} * kD * 2;
+    if (overlap(out, n_tokens * kRow, q, 2 * (n_tokens - 1) * q_token_stride + kRow)) return GQA_ERR_BAD_POINTER;
     if (!workspace || !aligned(workspace, 256) ||
         workspace_bytes < gqa_attention_q8_workspace_bytes(params, batch, n_tokens, max_new))
         return GQA_ERR_WORKSPACE;

@@ -87,16 +87,18 @@ hipError_t launch_q8_attention(const Q8AttnArgs& a, int format, hipStream_t stre
 
 constexpr int32_t kQ8MaxBatch = 32768;     // sequences that the counters at a workspace's start are for
 
-// A chunk of more than kQ8StreamMax tokens of one sequence goes to the tile kernel.
+// A chunk of more than kQ8StreamMax tokens of one sequence goes to the tile kernel: 16 tokens are the 64
+// columns whose sums fit a wave's registers.
 constexpr int kQ8StreamMax = 16;
 constexpr int kQ8TileTokens = 64;
 
-constexpr int kQ8TileWgsPerCu = 1;
+constexpr int kQ8TileWgsPerCu = 1;         // (eight waves of 256 registers fill a CU)
 
-// Waves of the stream kernel for each CU: one per SIMD.  (More of them read slower: HBM serves fewer
-// streams at once faster.)  Steps of a wave's ring in LDS (8 KB each).
+// Waves of the stream kernel for each CU: one per SIMD.  HBM serves fewer streams at once faster: shuffled
+// 2 KB rows copied to LDS by 4, 6 and 8 waves a CU come at 6.85, 6.68 and 6.32 TB/s.  Steps of a wave's
+// ring in LDS (8 KB each); a fourth is no faster.
 constexpr int kQ8WavesPerCu = 4;
-__host__ __device__ constexpr int q8_ring(int) { return 3; }
+constexpr int kQ8Ring = 3;
 
 // Columns (token, head) of a stream workgroup in tiles of 16: 4 tokens x 4 heads each.
 __host__ __device__ constexpr int q8_stream_tiles(int max_new) { return max_new <= 4 ? 1 : max_new <= 8 ? 2 : 4; }

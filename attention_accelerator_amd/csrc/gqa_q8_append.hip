@@ -16,6 +16,11 @@
 //
 // The workgroup takes its KV heads in turn, the next one's rows requested before this one's are worked
 // on; the sines and cosines of a token's 64 pairs, a third of the arithmetic, are formed once.
+//
+// A small step is one chain of dependent loads (slots; rows, positions, scales) behind a launch: 6 us for
+// 64 single tokens, 9 for 24 sequences with 1023 rows.  16384 rows take 39 us, 2.6 TB/s read and
+// written, where a copy takes 21: at 160 registers three workgroups share a CU, too few to hide that
+// chain (the kernel without its row loads, stores and sines still takes 23 us).
 #include "gqa_device.h"
 #include "gqa_internal.h"
 #include "gqa_q8.h"
@@ -25,6 +30,7 @@ namespace gqa {
 namespace {
 
 constexpr int kApWin = 16;                 // tokens of a window
+constexpr int kApSkip = 8 * kWave;          // skipped tokens passed at a time
 constexpr int kApRows = 2 * kApWin;        // rows a workgroup may read: the window's, and what ends its last run
 
 // The smallest power of two s with s * qmax >= a, at least 2^-126 (a finite, >= 0).  qmax is
@@ -166,6 +172,13 @@ __global__ __launch_bounds__(256) void q8_append_kernel(Q8AppendArgs a, int head
             const int32_t slot = t >= 0 && t < a.n_tokens ? a.slots[t] : -1;
             return slot >= 0 && slot < slots_end ? slot : -1;
         };
+        // Past skipped tokens, eight loads a lane at a time (a padded step may end in thousands of them).
+        auto none_of = [&](int64_t t) {
+            int32_t top = -1;
+#pragma unroll
+            for (int j = 0; j < kApSkip / kWave; ++j) top = max(top, slot_of(t + j * kWave + tid));
+            return !__any(top >= 0);
+        };
         // Lanes 0 .. 15: the window; 16 .. 31: the tokens before it; 32 .. 47: the ones behind.
         const int64_t t_of = tid < kApWin ? t0 + tid : tid < 2 * kApWin ? t0 + tid - 2 * kApWin : t0 + tid - kApWin;
         const int32_t slot = tid < 3 * kApWin ? slot_of(t_of) : -1;
@@ -175,7 +188,9 @@ __global__ __launch_bounds__(256) void q8_append_kernel(Q8AppendArgs a, int head
         if (in) {
             const uint32_t prev = static_cast<uint32_t>(valid >> kApWin) & 0xffffu;
             if (prev) before = __shfl(slot, kApWin + 31 - __clz(prev)) >> 4;
-            for (int64_t t = t0 - kApWin; !prev && before < 0 && t > 0; t -= kWave) {
+            for (int64_t t = t0 - kApWin; !prev && before < 0; t -= kWave) {
+                while (t > 0 && none_of(t - kApSkip)) t -= kApSkip;
+                if (t <= 0) break;
                 const int32_t s = slot_of(t - kWave + tid);
                 const uint64_t v = __ballot(s >= 0);
                 if (v) before = __shfl(s, 63 - __clzll(v)) >> 4;
@@ -214,7 +229,9 @@ __global__ __launch_bounds__(256) void q8_append_kernel(Q8AppendArgs a, int head
                 }
                 count += __popcll(more);
                 t += t == t0 + kApWin ? kApWin : kWave;
-                if (stop || count >= kApRows || t >= a.n_tokens) break;
+                if (stop || count >= kApRows) break;
+                while (t < a.n_tokens && none_of(t)) t += kApSkip;
+                if (t >= a.n_tokens) break;
                 s = slot_of(t + tid);
             }
             count = min(count, kApRows);
@@ -350,8 +367,9 @@ __global__ __launch_bounds__(256) void q8_append_kernel(Q8AppendArgs a, int head
 
 template <int kFmt>
 static hipError_t launch_append(const Q8AppendArgs& a, hipStream_t stream) {
-    // A workgroup for each window and head while that leaves CUs idle (a step's latency is one chain of
-    // loads), four heads in turn where there are several rounds of workgroups.
+    // A workgroup for each window and head while that leaves CUs idle, four heads in turn where there are
+    // several rounds of workgroups.  A call in us with 1 and 4 heads in turn: 64 windows 10.4 and 15.2,
+    // 1024 windows 60.8 and 43.5 (2 heads: 46.6).
     const int64_t windows = (static_cast<int64_t>(a.n_tokens) + kApWin - 1) / kApWin;
     const int heads = windows * kHkv <= 2048 ? 1 : 4;
     hipLaunchKernelGGL((q8_append_kernel<kFmt>), dim3(static_cast<unsigned>(windows * (kHkv / heads))), dim3(256), 0, stream, a,

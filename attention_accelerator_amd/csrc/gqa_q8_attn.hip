@@ -613,10 +613,15 @@ __device__ __forceinline__ void merge_token(const Q8AttnArgs& a, int n, RowOf ro
 //
 // The eight waves of a range are neighbours, one on each XCD, and read the eight heads' parts of the
 // same blocks at about the same time: HBM sees blocks of 16 KB, not 2.
+//
+// HBM bounds it: 64 sequences of 512..8192 keys, 661 MB, take 111 us, 6.0 TB/s; 8 of 131072, 2.16 GB, 336,
+// 6.4 TB/s.  One wave reads a step's eight operands together, before its arithmetic (left in place, each
+// waits for LDS: 113 -> 122 us for 8 tokens a sequence).  A single sequence of 4096 keys takes 13 us, its
+// ranges 4 steps long: a chain of lengths, ids, scales and keys, and the merge's.
 template <int kFmt, int kTiles, bool kOne>
 __global__ __launch_bounds__(kWave) __attribute__((amdgpu_waves_per_eu(1)))
 void q8_stream_kernel(Q8AttnArgs a) {
-    constexpr int kRing = q8_ring(kTiles);
+    constexpr int kRing = kQ8Ring;
     constexpr int kCopies = 8;                     // memory operations of a step's copies
     constexpr int kBatches = kRing + 1;            // the work's, up to kRing - 1 after it, and the next ids
     __shared__ __align__(4096) uint8_t s_ring[kRing][2][kQ8PlaneB];    // [buffer][K, V]

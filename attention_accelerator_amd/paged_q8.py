@@ -100,7 +100,7 @@ def paged_plan(cached: torch.Tensor, n_new: torch.Tensor, free_blocks: torch.Ten
     block_table    [B, max_blocks] int32 (rows contiguous), new blocks' entries written in place
     n_rows         token rows of the step, at least n_new's sum (more: padded rows)
     out            a PagedPlan to write into (for captured graphs); no tensor of it may overlap an
-                   input
+                   input or another one
     Returns the lengths with the new tokens (0: refused), the ragged row offsets, each row's slot (-1:
     refused or padding) and position, and what is left of the stack.  A request is granted whole or
     refused whole, first come, first served; refused are those the stack does not cover, and
@@ -182,7 +182,7 @@ def kv_append_q8(k_new: torch.Tensor, v_new: torch.Tensor, pool: Q8Pool, slot_ma
     positions  [N] int32 (may be None without rope_k)
     A block's scale is a power of two that covers its rows; where a row appended behind others needs a
     larger one, the rows before it are requantised.  The tokens of one block have to follow each
-    other in the call (skipped ones aside), each slot at most once, and no two sequences may append to one block."""
+    other in the call, row after row (skipped ones aside), each slot at most once, and no two sequences may append to one block."""
     k_new, v_new = _rows(k_new, "k_new", N_KV_HEADS, 8), _rows(v_new, "v_new", N_KV_HEADS, 8)
     n, device = k_new.shape[0], k_new.device
     if v_new.shape[0] != n or v_new.device != device:
@@ -224,7 +224,8 @@ class PreparedAttentionQ8:
     """A gqa_attention_q8 call with every argument bound once, for loops that repeat the same step
     (the tensors' values may change between calls): calling it issues the launches on the current
     stream with no checks or allocation.  The tensors passed in must stay alive while it is used.
-    Its workspace is its own: calls of one object must be ordered (one stream)."""
+    Its workspace is its own, cleared on the stream it is made on: that and the calls of one object
+    must be ordered (one stream, or events)."""
 
     def __init__(self, q: torch.Tensor, pool: Q8Pool, block_table: torch.Tensor, seq_len: torch.Tensor,
                  cu_new: Optional[torch.Tensor] = None, *, max_new: Optional[int] = None, rope_q: bool = True,
@@ -287,6 +288,7 @@ def gqa_attention_q8(q: torch.Tensor, pool: Q8Pool, block_table: torch.Tensor, s
                  streamed kernel; a tight bound keeps idle launches out
     workspace    from new_attention_q8_workspace, for calls up to its sizes (else one is made for the call);
                  calls that share it must be ordered
+    out          may not overlap q
     Returns out [N, 32, 128]; rows behind cu_new[B] are left as they were in `out`."""
     q = _rows(q, "q", N_Q_HEADS, 16)
     if isinstance(block_table, torch.Tensor):

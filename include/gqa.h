@@ -281,8 +281,8 @@ int gqa_kv_append_bf16(const gqa_params_t* params, const uint16_t* k_new, const 
  * served: it is granted where the needs of the requests up to it fit (and always where it
  * needs none), else refused whole: its entries, slots and length as above.  Refused too:
  * negative values, more than 16 * max_blocks positions, rows past n_rows (these count for no
- * other request).  All arrays are device memory, and no output may overlap an input (the
- * block table's kept entries are read; n_free_out is not n_free).  n_new[b] == 0 is a request at
+ * other request).  All arrays are device memory, and no output may overlap an input or
+ * another output (the block table's kept entries are read; n_free_out is not n_free).  n_new[b] == 0 is a request at
  * rest. */
 int gqa_paged_plan(const int32_t* cached, const int32_t* n_new, int32_t batch, const int32_t* free_blocks,
                    const int32_t* n_free, int32_t free_capacity, int32_t* block_table, int64_t table_stride,
@@ -319,8 +319,9 @@ typedef struct gqa_q8_kv {
  * present scale, and where it grows the rows before it are requantised (code * old / new).  Codes
  * are rounded to nearest even and saturate; a NaN becomes e4m3's NaN, 0 in int8.  A present scale
  * that is not a positive finite number counts as 0.  The tokens of one block have to follow each
- * other in the call (skipped ones aside), each slot at most once, and no two sequences may write one block: a block is
- * read, scaled and written by one workgroup.  positions may be NULL without GQA_ROPE_K. */
+ * other in the call, row after row (skipped tokens aside), each slot at most once, and no two
+ * sequences may write one block: a block is read, scaled and written by one workgroup.  No two elements of a pool may share a place (strides of an
+ * expanded pool: GQA_ERR_INVALID_CONFIG).  positions may be NULL without GQA_ROPE_K. */
 int gqa_kv_append_q8(const gqa_params_t* params, const uint16_t* k_new, int64_t k_token_stride,
                      const uint16_t* v_new, int64_t v_token_stride, void* k_pool, void* v_pool, float* k_scale,
                      float* v_scale, const gqa_q8_kv_t* kv, const int32_t* slots, const int32_t* positions,
@@ -332,7 +333,7 @@ int gqa_kv_append_q8(const gqa_params_t* params, const uint16_t* k_new, int64_t 
  * position when GQA_ROPE_Q; the cache holds post-RoPE K (GQA_ROPE_K is rejected).
  *   q      row r, head i at r*q_token_stride + 128 i elements (stride a multiple of 8, 16-byte
  *          aligned); n_tokens rows
- *   out    [n_tokens][32][128]; rows that belong to no sequence are left as they were
+ *   out    [n_tokens][32][128], apart from q; rows that belong to no sequence are left as they were
  *   max_new  at least every sequence's rows (a host bound; it chooses the kernels)
  *   workspace  gqa_attention_q8_workspace_bytes bytes, 256-byte aligned, cleared once by
  *          gqa_attention_q8_workspace_init before its first call (its counters read zero between

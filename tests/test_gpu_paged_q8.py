@@ -254,6 +254,17 @@ def test_append_token_by_token(dev, fmt):
     assert (off <= (quantum if fmt == "int8" else torch.maximum(step, quantum * 2.0 ** -10) + quantum * 2.0 ** -9)).all()
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("gaps", [(0, 20, 40), (3, 530, 1500), (700, 15, 513), (1100, 1, 2000)])
+def test_append_long_stretches_of_skipped_tokens(dev, fmt, gaps):
+    """Tokens of one block far apart, and skipped ones before and behind them."""
+    slots = [-1] * gaps[0] + [19, 20] + [-1] * gaps[1] + [21, 47] + [-1] * gaps[1] + [54, 55] + [-1] * gaps[2]
+    gen = torch.Generator().manual_seed(sum(gaps))
+    pool = random_pool(4, fmt, gen, spread=4)
+    k, v = (torch.randn((len(slots), 8, 128), generator=gen).to(torch.bfloat16) for _ in range(2))
+    check_append(dev, pool, k, v, slots, list(range(len(slots))), fmt)
+
+
 def test_append_nothing(dev):
     pool = gqa.new_q8_pool(2, torch.int8, dev)
     x = torch.zeros((0, 8, 128), dtype=torch.bfloat16, device=dev)
@@ -458,6 +469,73 @@ def test_attention_on_another_stream_and_repeats(dev):
         torch.cuda.synchronize()
         for c, w in zip(calls, wants):
             assert torch.equal(c.out, w)
+
+
+@pytest.mark.parametrize("news,lens,stream_wgs", [
+    ([1, 1], [5003, 3100], 0), ([1, 1], [5003, 3100], 16), ([7], [4111], 16), ([2, 16], [2500, 1999], 16),
+    ([100], [4500], 16), ([33], [6001], 0),
+])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_attention_long_ranges(dev, fmt, news, lens, stream_wgs):
+    """Ranges and runs of many steps: block ids and scales come in several batches."""
+    q, pool, table, cu = make_batch(fmt, news, lens, seed=lens[0])
+    got = run_attention(dev, q, pool, table, lens, cu, max_new=max(news), params=gqa.make_params(stream_wgs=stream_wgs))
+    want, bound = _q8.attend(q, _q8.codes64(pool[0]), _q8.codes64(pool[1]), pool[2], pool[3], table, lens, cu)
+    assert_close(got, want, bound, f"{fmt} {news} {lens}")
+
+
+@pytest.mark.parametrize("most", [1, 2, 20])
+def test_attention_many_sequences(dev, most):
+    """More sequences than a wave has lanes, some of them empty or without new rows, one odd one."""
+    r = random.Random(most)
+    news = [r.choice([0, 1, 1, r.randint(1, most)]) if most > 1 else 1 for _ in range(150)]
+    lens = [n + r.choice([0, 3, r.randint(0, 70), r.randint(0, 260)]) for n in news]
+    q, pool, table, cu = make_batch("int8", news, lens, seed=most)
+    bad = news.index(max(news), 70)
+    lens[bad] = news[bad] - 1
+    got = run_attention(dev, q, pool, table, lens, cu, max_new=most)
+    assert got[cu[bad]:cu[bad + 1]].isnan().all()
+    lens[bad] = news[bad]
+    want, bound = _q8.attend(q, _q8.codes64(pool[0]), _q8.codes64(pool[1]), pool[2], pool[3], table, lens, cu)
+    keep = [t for t in range(cu[-1]) if not cu[bad] <= t < cu[bad + 1]]
+    assert_close(got[keep], want[keep], bound[keep], str(most))
+
+
+def test_attention_one_workspace_for_all(dev):
+    """Calls of every kind in turn on one workspace, and rows behind the last sequence."""
+    batches = [([1, 1, 1], [700, 40, 1300]), ([40, 1], [900, 33]), ([8, 3], [500, 777]), ([1], [3000]), ([1] * 70, [90] * 70)]
+    ws = gqa.new_attention_q8_workspace(70, 200, 64, dev)
+    calls = []
+    for i, (news, lens) in enumerate(batches):
+        q, pool, table, cu = make_batch("e4m3", news, lens, seed=40 + i)
+        q = torch.cat((q, torch.full((3, 32, 128), float("nan"), dtype=torch.bfloat16)))
+        out = torch.full(q.shape, 5.0, dtype=torch.bfloat16, device=dev)
+        args = (q.to(dev), to_dev(pool, dev), i32(table, dev), i32(lens, dev), i32(cu, dev))
+        calls.append((gqa.PreparedAttentionQ8(*args, max_new=max(news), workspace=ws, out=out), cu[-1],
+                      gqa.gqa_attention_q8(*args, max_new=max(news))[:cu[-1]].clone()))
+    for turn in range(3):
+        for call, rows, want in calls[turn:] + calls[:turn]:
+            call.out[:rows] = 0
+            assert torch.equal(call()[:rows], want) and (call.out[rows:] == 5).all()
+
+
+def test_attention_mixed_step_graph_replays(dev):
+    """A mixed step captured with its workspace made inside, replayed with new values and eager calls between."""
+    news, lens = [40, 1, 7, 1], [300, 500, 90, 64]
+    q, pool, table, cu = make_batch("int8", news, lens, seed=9)
+    gen = torch.Generator().manual_seed(10)
+    args = [q.to(dev), to_dev(pool, dev), i32(table, dev), i32(lens, dev), i32(cu, dev)]
+    gqa.gqa_attention_q8(*args, max_new=40)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = gqa.gqa_attention_q8(*args, max_new=40)
+    for turn in range(5):
+        args[0].copy_(torch.randn(q.shape, generator=gen).to(torch.bfloat16))
+        args[3].copy_(i32([n - 3 * turn for n in lens], dev))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, gqa.gqa_attention_q8(*args, max_new=40))
 
 
 # ------------------------------------------------------------------------------------ a serving run

@@ -145,6 +145,47 @@ def test_python_refuses_cpu_tensors():
         gqa.gqa_attention_q8(torch.zeros((2, 32, 128), dtype=torch.bfloat16), pool, torch.zeros((2, 4), dtype=torch.int32), i)
 
 
+# -- arrays that share a place
+
+@pytest.mark.parametrize("change", [
+    dict(cu=6 * A + 4), dict(slots=9 * A + 28), dict(n_free_out=8 * A + 12), dict(seq_len=A + 4), dict(positions=5 * A + 28),
+    dict(free=5 * A - 4), dict(n_free=5 * A + 4), dict(table=3 * A + 28), dict(positions=8 * A - 4), dict(n_free_out=10 * A, cu=10 * A - 8),
+])
+def test_plan_refuses_shared_places(change):
+    assert plan_call(**change) == BAD_PTR
+
+
+@pytest.mark.parametrize("change", [
+    dict(block_stride=0), dict(head_stride=0), dict(head_stride=128), dict(block_stride=8192), dict(pos_stride=2048),
+    dict(scale_head_stride=0), dict(scale_block_stride=0), dict(scale_block_stride=7), dict(scale_block_stride=1, scale_head_stride=9),
+    dict(block_stride=1 << 62, n_blocks=1 << 20),
+])
+def test_append_refuses_expanded_pools(change):
+    assert append_call(lay=layout(**change)) == BAD_CFG
+
+
+@pytest.mark.parametrize("change", [dict(k=4 * A), dict(ks=6 * A)])
+def test_append_refuses_one_pool_for_both(change):
+    assert append_call(**change) == BAD_PTR
+
+
+@pytest.mark.parametrize("out", [A, A + 8192, A + 4 * 8192 - 8, A - 8])
+def test_attention_refuses_out_over_q(out):
+    assert attend_call(out=out) == BAD_PTR
+
+
+def test_workspace_init_refusals():
+    init = _lib.lib().gqa_attention_q8_workspace_init
+    assert init(None, 1 << 30, None) == BAD_WS
+    assert init(A + 128, 1 << 30, None) == BAD_WS
+    assert init(A, 1024, None) == BAD_WS
+
+
+def test_batches_beyond_the_counters():
+    assert gqa.attention_q8_workspace_bytes(32769, 40000, 1) == 0 < gqa.attention_q8_workspace_bytes(32768, 40000, 1)
+    assert attend_call(batch=32769, n=40000) == BAD_CFG
+
+
 # -- the plain forms themselves, against torch's own conversions and written-out results
 
 def test_plain_e4m3_rounds_as_torch():
