@@ -827,6 +827,11 @@ int32_t q8_tile_wgs(const gqa_params_t* p) {
 // call: what one call's partials lie in is never another's counters.
 constexpr size_t kQ8CounterBytes = size_t{kQ8MaxBatch} * kHkv * sizeof(uint32_t);
 
+// ... then an entry for each range.
+size_t q8_cut_bytes(const gqa_params_t* p) {
+    return align_up(static_cast<size_t>(q8_stream_waves(p) / kHkv) * sizeof(Q8CutSeq), 256);
+}
+
 // Partial rows of the stream kernel (two pieces of every range), then of the tile kernel.
 int64_t q8_stream_rows(const gqa_params_t* p, int32_t max_new) {
     return int64_t{2} * q8_stream_waves(p) * (max_new == 1 ? kGroup : 16 * q8_stream_tiles(max_new));
@@ -919,7 +924,7 @@ int gqa_kv_append_q8(const gqa_params_t* params, const uint16_t* k_new, int64_t 
 size_t gqa_attention_q8_workspace_bytes(const gqa_params_t* params, int32_t batch, int32_t n_tokens, int32_t max_new) {
     if (!params || !geometry_ok(params) || batch <= 0 || batch > kQ8MaxBatch || n_tokens <= 0 || max_new <= 0) return 0;
     const size_t rows = static_cast<size_t>(q8_rows(params, max_new));
-    return kQ8CounterBytes + align_up(rows * kD * sizeof(float), 256) + align_up(rows * sizeof(float4), 256);
+    return kQ8CounterBytes + q8_cut_bytes(params) + align_up(rows * kD * sizeof(float), 256) + align_up(rows * sizeof(float4), 256);
 }
 
 int gqa_attention_q8_workspace_init(void* workspace, size_t workspace_bytes, void* stream) {
@@ -959,7 +964,8 @@ int gqa_attention_q8(const gqa_params_t* params, const uint16_t* q, int64_t q_to
     a.cu = cu_new;
     a.out = out;
     a.counters = static_cast<uint32_t*>(workspace);
-    char* partials = static_cast<char*>(workspace) + kQ8CounterBytes;
+    a.cut_seqs = reinterpret_cast<Q8CutSeq*>(static_cast<char*>(workspace) + kQ8CounterBytes);
+    char* partials = static_cast<char*>(workspace) + kQ8CounterBytes + q8_cut_bytes(params);
     a.part_o = reinterpret_cast<float*>(partials);
     a.part_ml = reinterpret_cast<float4*>(partials + align_up(static_cast<size_t>(rows) * kD * sizeof(float), 256));
     a.tile_slot0 = q8_stream_rows(params, max_new);

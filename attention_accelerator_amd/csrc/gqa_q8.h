@@ -38,6 +38,12 @@ struct Q8AppendArgs {
     RopeTable rope_table;
 };
 
+// The sequence that begins in a range and goes on behind it (n = 0: none): its steps there, and a range's.
+struct Q8CutSeq {
+    int32_t row0, n;
+    int64_t left, per;
+};
+
 struct Q8AttnArgs {
     Q8Pool pool;
     const uint16_t* q;
@@ -48,6 +54,7 @@ struct Q8AttnArgs {
     uint16_t* out;
     uint32_t* counters;                    // [8][kQ8MaxBatch] pieces written (the heads' far apart: counts in one
                                            // cache line wait for each other); 0 between calls
+    Q8CutSeq* cut_seqs;                    // of each range; not of one-token calls
     float* part_o;                         // partial O rows, 128 floats each
     float4* part_ml;                       // (m, M, l, -) of each partial row
     int64_t tile_slot0;                    // first partial row of the tile kernel's part

@@ -433,13 +433,15 @@ struct Q8Window {
     int b0;
     Q8Seq seq;                             // this lane's
     int steps;                             // 0: not in the stream
+    bool bad;                              // rows to be NaN: its lengths break the rules
 
     __device__ __forceinline__ void load(const Q8AttnArgs& a, int first, int lane) {
         b0 = first;
         seq = Q8Seq{0, 0, 0};
         steps = 0;
-        if (b0 + lane < a.batch && q8_seq(a, b0 + lane, seq) && seq.n <= kQ8StreamMax)
-            steps = (seq.start + seq.n + kQ8Step - 1) / kQ8Step;
+        const bool good = b0 + lane < a.batch && q8_seq(a, b0 + lane, seq);
+        if (good && seq.n <= kQ8StreamMax) steps = (seq.start + seq.n + kQ8Step - 1) / kQ8Step;
+        bad = !good && seq.n > 0;
     }
 };
 
@@ -487,9 +489,9 @@ struct Q8Shared {
 
 // NaN rows (of KV head h) for a sequence whose lengths break the rules, or that has more than max_new
 // rows; none where its offsets do.
-__device__ __forceinline__ void write_nan(const Q8AttnArgs& a, const Q8Seq& sq, int h, int lane, int first, int stride) {
+__device__ __forceinline__ void write_nan(const Q8AttnArgs& a, const Q8Seq& sq, int h, int lane) {
     if (sq.row0 < 0 || sq.n <= 0 || static_cast<int64_t>(sq.row0) + sq.n > a.n_tokens) return;
-    for (int t = first; t < sq.n; t += stride) {
+    for (int t = 0; t < sq.n; ++t) {
         uint32_t* row = reinterpret_cast<uint32_t*>(a.out) + ((static_cast<int64_t>(sq.row0) + t) * kHq + kGroup * h) * (kD / 2);
         for (int i = lane; i < kGroup * kD / 2; i += kWave) row[i] = 0x7fc07fc0u;
     }
@@ -607,9 +609,8 @@ __device__ __forceinline__ void merge_token(const Q8AttnArgs& a, int n, RowOf ro
 // that enters wave w's range from the one before, 2w + 1 of the one that leaves it.
 //
 // With one new token for each sequence (kOne) the merge is part of this kernel: the last of a sequence's
-// pieces to be written, by a counter in the workspace that it puts back to zero, merges them all, and
-// lengths that break the rules get their NaN rows here.  Of more tokens' partials one wave would
-// read up to megabytes: they have a launch of their own.
+// pieces to be written, by a counter in the workspace that it puts back to zero, merges them all.  Of
+// more tokens' partials one wave would read up to megabytes: they have a launch of their own.
 //
 // The eight waves of a range are neighbours, one on each XCD, and read the eight heads' parts of the
 // same blocks at about the same time: HBM sees blocks of 16 KB, not 2.
@@ -641,15 +642,13 @@ void q8_stream_kernel(Q8AttnArgs a) {
         win.load(a, b0, lane);
         all += static_cast<uint32_t>(lane_value(wave_scan(win.steps), kWave - 1));
         seqs += __popcll(__ballot(win.steps > 0));
-        if constexpr (kOne) {                      // the wave of (b, h): b by the ranges in turn
-            uint64_t bad = __ballot(win.steps == 0 && win.seq.n > 0);
-            for (; bad; bad &= bad - 1) {
-                const int at = __builtin_ctzll(bad);
-                if ((b0 + at) % (a.stream_waves / kHkv) != wave / kHkv) continue;
-                write_nan(a, Q8Seq{lane_value(win.seq.row0, at), lane_value(win.seq.n, at), 0}, h, lane, 0, 1);
-            }
+        for (uint64_t bad = __ballot(win.bad); bad; bad &= bad - 1) {      // the wave of (b, h): b by the ranges in turn
+            const int at = __builtin_ctzll(bad);
+            if ((b0 + at) % (a.stream_waves / kHkv) != wave / kHkv) continue;
+            write_nan(a, Q8Seq{lane_value(win.seq.row0, at), lane_value(win.seq.n, at), 0}, h, lane);
         }
     }
+    if (!kOne && h == 0 && lane == 0) a.cut_seqs[wave / kHkv] = Q8CutSeq{0, 0, 0, 0};
     const Q8Cut cut(all, seqs, a.stream_waves / kHkv);
     int64_t x = wave / kHkv * cut.per;             // next position
     const int64_t x_end = min(x + cut.per, cut.total);
@@ -786,7 +785,7 @@ void q8_stream_kernel(Q8AttnArgs a) {
     ids(cur, cur.first / 32);
     int slot = 0, buf = 0;
     // The piece cur, of at most 4 kNow tokens.  The kernel of four column tiles meets many single tokens
-    // (decodes beside prompt chunks) and works on their one tile alone: 87 -> 70 us for 22 decodes and two
+    // (decodes beside prompt chunks) and works on their one tile alone: 87 -> 71 us for 22 decodes and two
     // chunks of 301 tokens.  (Two tiles stay within the time of the reads: 113 us either way for 64
     // sequences of 8 tokens over 512..8192.)
     auto work = [&](auto now) {
@@ -846,6 +845,8 @@ void q8_stream_kernel(Q8AttnArgs a) {
             if constexpr (kOne) {                  // counted when the wave has no more to request
                 const int r0 = cut.first_range(cur.at), n = cut.last_range(cur.at, cur.steps) - r0 + 1;
                 (cur.first == 0 ? leaving : entering) = Part{cur.b, cur.row0, r0, n};
+            } else if (cur.first == 0 && h == 0 && lane == 0) {
+                a.cut_seqs[wave / kHkv] = Q8CutSeq{cur.row0, cur.n, cur.at + cur.steps - x_end, cut.per};
             }
         }
     };
@@ -1172,12 +1173,16 @@ __global__ __launch_bounds__(kTileWaves * kWave) __attribute__((amdgpu_waves_per
 }
 
 // ---------------------------------------------------------------------------------------------
-// Merge kernel: a wave for each of the tokens of (sequence, KV head) in the stream, up to 16, the first
-// `stream` workgroups; then kTileMergeWaves for each (tile, KV head), its tokens in turn.  A KV head's
-// waves run on one XCD, the one whose waves wrote its partials (its L2 may still hold them).
+// Merge kernel: up to kRangeMergeWaves for each (range, KV head), which share the tokens of the sequence that
+// begins in the range and goes on behind it: the first `stream` workgroups.  (The stream kernel names that
+// sequence in the workspace.  Found here, by every wave through all lengths, it took 470 us of 1240 for 4096
+// sequences of 2 tokens over 512, now 830.)  Then kTileMergeWaves for each (tile, KV head), its tokens in
+// turn.  A KV head's waves run on one XCD, the one whose waves wrote its partials (its L2 may still hold
+// them).
+constexpr int kRangeMergeWaves = 4;          // (1, 2, 8: 122, 116, 114 us for 64 sequences of 8 tokens; 4: 114)
 constexpr int kTileMergeWaves = 32;          // (16: 1.2 us more for two chunks of 301 tokens)
 
-__global__ __launch_bounds__(kWave) void q8_merge_kernel(Q8AttnArgs a, int cols, int stream, int toks) {
+__global__ __launch_bounds__(kWave) void q8_merge_kernel(Q8AttnArgs a, int cols, int stream, int waves) {
     const int lane = threadIdx.x;
     const int h = blockIdx.x % kHkv;
     auto out_of = [&](int row) { return a.out + (static_cast<int64_t>(row) * kHq + kGroup * h) * kD; };
@@ -1202,36 +1207,16 @@ __global__ __launch_bounds__(kWave) void q8_merge_kernel(Q8AttnArgs a, int cols,
         }
         return;
     }
-    const int tok = blockIdx.x / kHkv % toks, b = blockIdx.x / kHkv / toks;
-    Q8Seq sq;
-    if (!q8_seq(a, b, sq)) {
-        write_nan(a, sq, h, lane, tok, toks);
-        return;
+    const int first = blockIdx.x / kHkv % waves, r0 = blockIdx.x / kHkv / waves;
+    const Q8CutSeq seq = a.cut_seqs[r0];
+    if (first >= seq.n) return;
+    const int pieces = 1 + static_cast<int>((seq.left + seq.per - 1) / seq.per);
+    for (int tok = first; tok < seq.n; tok += waves) {
+        auto row_of = [&](int i) {
+            return (2 * (static_cast<int64_t>(r0 + i) * kHkv + h) + (i == 0 ? 1 : 0)) * static_cast<int64_t>(cols) + kGroup * tok;
+        };
+        merge_token<false>(a, pieces, row_of, out_of(seq.row0 + tok), lane);
     }
-    if (sq.n > kQ8StreamMax || tok >= sq.n) return;
-    // The sequence's place in the stream.
-    int64_t before = 0, all = 0;
-    int steps = 0, seqs = 0, seqs_before = 0;
-    Q8Window win;
-    for (int b0 = 0; b0 < a.batch; b0 += kWave) {
-        win.load(a, b0, lane);
-        const uint32_t upto = wave_scan(win.steps);
-        const uint64_t some = __ballot(win.steps > 0);
-        if (b - b0 >= 0 && b - b0 < kWave) {
-            steps = lane_value(win.steps, b - b0);
-            before = all + static_cast<uint32_t>(lane_value(upto, b - b0)) - steps;
-            seqs_before = seqs + __popcll(some & ((1ull << (b - b0)) - 1));
-        }
-        all += static_cast<uint32_t>(lane_value(upto, kWave - 1));
-        seqs += __popcll(some);
-    }
-    if (steps == 0) return;
-    const Q8Cut cut(all, seqs, a.stream_waves / kHkv);
-    const int64_t x = before + static_cast<int64_t>(cut.lead) * (seqs_before + 1);
-    const int64_t r0 = cut.first_range(x), r1 = cut.last_range(x, steps);
-    if (r0 == r1) return;                          // one piece: written already
-    auto row_of = [&](int i) { return (2 * ((r0 + i) * kHkv + h) + (i == 0 ? 1 : 0)) * static_cast<int64_t>(cols) + kGroup * tok; };
-    merge_token<false>(a, static_cast<int>(r1 - r0 + 1), row_of, out_of(sq.row0 + tok), lane);
 }
 
 template <int kFmt, int kTiles, bool kOne = false>
@@ -1252,12 +1237,12 @@ static hipError_t launch_attention(const Q8AttnArgs& a, hipStream_t stream) {
     if (tiles == 1) launch_stream<kFmt, 1>(a, stream);
     else if (tiles == 2) launch_stream<kFmt, 2>(a, stream);
     else launch_stream<kFmt, 4>(a, stream);
-    const int toks = a.max_new < kQ8StreamMax ? a.max_new : kQ8StreamMax;
-    const int of_stream = a.batch * kHkv * toks;
+    const int waves = a.max_new < kRangeMergeWaves ? a.max_new : kRangeMergeWaves;
+    const int of_stream = a.stream_waves * waves;
     // (runs > 1 only where the tiles and heads are at most half of the workgroups)
     const int of_tiles = a.max_new > kQ8StreamMax ? a.tile_wgs / 2 / kHkv * kHkv * kTileMergeWaves : 0;
     hipLaunchKernelGGL(q8_merge_kernel, dim3(static_cast<unsigned>(of_stream + of_tiles)), dim3(kWave), 0, stream, a, 16 * tiles,
-                       of_stream, toks);
+                       of_stream, waves);
     return hipGetLastError();
 }
 
