@@ -648,7 +648,9 @@ void q8_stream_kernel(Q8AttnArgs a) {
             write_nan(a, Q8Seq{lane_value(win.seq.row0, at), lane_value(win.seq.n, at), 0}, h, lane);
         }
     }
-    if (!kOne && h == 0 && lane == 0) a.cut_seqs[wave / kHkv] = Q8CutSeq{0, 0, 0, 0};
+    // (all lanes store the same: under a branch on the lane the compiler keeps the loop's uniform values in
+    // vector registers, 32 more)
+    if (!kOne && h == 0) a.cut_seqs[wave / kHkv] = Q8CutSeq{0, 0, 0, 0};
     const Q8Cut cut(all, seqs, a.stream_waves / kHkv);
     int64_t x = wave / kHkv * cut.per;             // next position
     const int64_t x_end = min(x + cut.per, cut.total);
@@ -785,7 +787,7 @@ void q8_stream_kernel(Q8AttnArgs a) {
     ids(cur, cur.first / 32);
     int slot = 0, buf = 0;
     // The piece cur, of at most 4 kNow tokens.  The kernel of four column tiles meets many single tokens
-    // (decodes beside prompt chunks) and works on their one tile alone: 87 -> 71 us for 22 decodes and two
+    // (decodes beside prompt chunks) and works on their one tile alone: 87 -> 68 us for 22 decodes and two
     // chunks of 301 tokens.  (Two tiles stay within the time of the reads: 113 us either way for 64
     // sequences of 8 tokens over 512..8192.)
     auto work = [&](auto now) {
@@ -845,12 +847,12 @@ void q8_stream_kernel(Q8AttnArgs a) {
             if constexpr (kOne) {                  // counted when the wave has no more to request
                 const int r0 = cut.first_range(cur.at), n = cut.last_range(cur.at, cur.steps) - r0 + 1;
                 (cur.first == 0 ? leaving : entering) = Part{cur.b, cur.row0, r0, n};
-            } else if (cur.first == 0 && h == 0 && lane == 0) {
-                a.cut_seqs[wave / kHkv] = Q8CutSeq{cur.row0, cur.n, cur.at + cur.steps - x_end, cut.per};
             }
         }
     };
     while (true) {
+        if (!kOne && cur.first == 0 && cur.end < cur.steps && h == 0)
+            a.cut_seqs[wave / kHkv] = Q8CutSeq{cur.row0, cur.n, cur.at + cur.steps - x_end, cut.per};
         if (kTiles == 4 && cur.n <= 4) work(std::integral_constant<int, 1>{});
         else work(std::integral_constant<int, kTiles>{});
         if (!have_next) break;
