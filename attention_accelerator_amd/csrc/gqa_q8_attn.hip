@@ -140,14 +140,20 @@ __device__ __forceinline__ const uint16_t* q_row(const Q8AttnArgs& a, int row, i
 }
 
 // cos and sin of `tokens` positions from `start` on, by `threads` threads (a token's 64 pairs by
-// 64 of them).
+// 64 of them): each thread's first from the angle, the ones after it turned on by the angle of its stride, in
+// double (16 turns keep 2^-48 of it; sines of every angle: 2 us more for 64 sequences of 8 tokens).
 __device__ __forceinline__ void fill_angles(const Q8AttnArgs& a, int start, int tokens, float2* cs, int tid, int threads) {
     if (!a.rope) return;
     const double f = a.rope_table.inv_freq[tid & 63];
-    for (int t = tid >> 6; t < tokens; t += threads >> 6) {
-        double s, c;
-        rope_sincos(start + t, f, s, c);
+    const int by = threads >> 6;
+    double s, c, turn_s = 0.0, turn_c = 1.0;
+    rope_sincos(start + (tid >> 6), f, s, c);
+    if (tokens > by) rope_sincos(by, f, turn_s, turn_c);
+    for (int t = tid >> 6; t < tokens; t += by) {
         cs[t * kPairs + (tid & 63)] = make_float2(static_cast<float>(c), static_cast<float>(s));
+        const double u = c * turn_c - s * turn_s;
+        s = s * turn_c + c * turn_s;
+        c = u;
     }
 }
 
@@ -891,18 +897,20 @@ void q8_stream_kernel(Q8AttnArgs a) {
 // KV head) per workgroup of 8 waves, 8 tokens (two column tiles) each.  Two waves share a SIMD: one's
 // products run under the other's exponentials.
 //
-// What bounds it is the issue of vector instructions (the exponentials and what is around them), so
-// the workgroup converts K and V to fp16 once for its eight waves: two steps (a stage) at a time,
-// each thread 16 codes of K and of V, read into registers while the stage before is worked on and
-// written to the other of two fp16 buffers behind it, with one barrier a stage.  4 sequences with
-// chunks of 512 tokens over 8192 take 309 us: 920 TFLOP/s of products.  (Codes in LDS that every wave
-// converts for itself: 348 us; only V as codes: 337; four waves of four column tiles, a SIMD each: 480.)
-// What is left is LDS: a wave reads 16 KB a step, its workgroup 128 KB in about 1024 of the step's 1200
-// clocks.  Where the tiles do not fill the workgroups their keys are
-// cut into runs.
+// The workgroup converts K and V to fp16 once for its eight waves, two steps (a stage) at a time:
+// each thread takes 16 codes of K and of V, read into registers a stage or two ahead, and writes them
+// to the other of two fp16 buffers, with one barrier a stage.  The first wave of a SIMD converts
+// at a stage's end and the second at its start: that keeps their products and exponentials apart (303 us
+// where both convert at the end: 308).  Where the tiles do not fill the workgroups their keys are cut
+// into runs.
+//
+// 4 sequences with chunks of 512 tokens over 8192 take 303 us: 937 TFLOP/s of products.  A step of 32 keys
+// takes a SIMD 2350 clocks: 1024 of products, about 1600 of vector issue (exponentials, sums, conversions), 1024
+// of the CU's LDS reads; the two waves overlap them only in part.  (Codes in LDS that every wave converts for
+// itself: 348 us; only V as codes: 337; four waves of four column tiles, a SIMD each: 480; the second wave
+// half a step behind the first, with three buffers: 357, it spills; higher priority for products: 323.)
 constexpr int kTileWaves = 8;
 constexpr int kTileCols = kQ8TileTokens * kGroup;
-constexpr int kTileKeys = 2 * kQ8Step;     // of a stage
 constexpr int kTileRowB = 2 * kD;          // bytes of a row in fp16
 constexpr int kTilePlaneB = kQ8Step * kTileRowB;       // K (or V) of a step in fp16
 constexpr int kTileMinRun = 8;             // steps of the shortest run
@@ -1047,6 +1055,7 @@ __global__ __launch_bounds__(kTileWaves * kWave) __attribute__((amdgpu_waves_per
     const uint32_t kdst = (row >> 5) * 2 * kTilePlaneB + row32 * kTileRowB + 16 * ((2 * chunk) ^ k_swizzle(row32));
     const uint32_t vdst = (row >> 5) * 2 * kTilePlaneB + kTilePlaneB + row32 * kTileRowB + 32 * (chunk ^ (row32 & 7));
     const uint32_t koff = k16_offset(lane), voff = v16_offset(lane);
+    const bool late = wv >= kTileWaves / 2;            // the second wave of each SIMD
     const int64_t items = static_cast<int64_t>(tiles) * kHkv * runs;
     for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
         const int h = static_cast<int>(item % kHkv);
@@ -1098,9 +1107,10 @@ __global__ __launch_bounds__(kTileWaves * kWave) __attribute__((amdgpu_waves_per
             request_ids(batches, table, first, n_blk, lane);
             wait_copies<0>();
         }
-        fill_angles(a, sq.start + tok0, tokens, s_cs, tid, kTileWaves * kWave);
         tile_barrier();
         read(0);
+        fill_angles(a, sq.start + tok0, tokens, s_cs, tid, kTileWaves * kWave);
+        tile_barrier();
         Q8State<kTiles> st;
         q8_f16x8 qop[kTiles][4];
         float qs[kTiles];
@@ -1114,11 +1124,17 @@ __global__ __launch_bounds__(kTileWaves * kWave) __attribute__((amdgpu_waves_per
         }
         st.clear();
         convert(0);
+        if (late && first + 2 < end) read(2);
         if (wv == 0) wait_copies<0>();             // the first batch's scales
         tile_barrier();
         for (int step0 = first; step0 < end; step0 += 2) {
             const bool more = step0 + 2 < end;
-            if (more) read(step0 + 2 - first);
+            if (late) {
+                if (more) convert(step0 + 2 - first);
+                if (step0 + 4 < end) read(step0 + 4 - first);
+            } else if (more) {
+                read(step0 + 2 - first);
+            }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int step = step0 + e;
@@ -1159,7 +1175,7 @@ __global__ __launch_bounds__(kTileWaves * kWave) __attribute__((amdgpu_waves_per
                         st.o[c][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[dt], p[c], st.o[c][dt], 0, 0, 0);
             }
             if (more) {
-                convert(step0 + 2 - first);
+                if (!late) convert(step0 + 2 - first);
                 if (wv == 0 && ((step0 + 2 - first) & 31) == 0) wait_copies<0>();      // the batch's scales
                 tile_barrier();
             }
