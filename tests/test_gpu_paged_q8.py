@@ -6,11 +6,14 @@ from __future__ import annotations
 
 import math
 import random
+import re
 
 import pytest
 import torch
 
 import attention_accelerator_amd as gqa
+from attention_accelerator_amd import _lib
+from conftest import ROOT
 import _q8
 
 pytestmark = pytest.mark.gpu
@@ -573,6 +576,30 @@ def test_serving_steps(dev, fmt):
         want, bound = _q8.attend(qkv[:, :32], plain[0], plain[1], scales[0], scales[1], t, lens, cu)
         assert_close(out.cpu()[:cu[-1]], want[:cu[-1]], bound[:cu[-1]], str(news))
         cached, n_free = plan.seq_len, plan.n_free
+
+
+def test_documented_ctypes_step(dev):
+    """The ctypes stub that the integration document gives for a step, run as written, against the
+    package's tensor calls, bit for bit."""
+    text = (ROOT / "INTEGRATION.md").read_text()
+    stub = [re.search(r"```python\n(.*?)```", text[text.index(s):], flags=re.S).group(1) for s in ("## 2.", "## 8.")]
+    src = "\n".join(stub).replace('"/path/to/attention_accelerator_amd/libgqa.so"', repr(str(_lib.LIB_PATH)))
+    ns: dict = {}
+    exec(compile(src, "INTEGRATION.md", "exec"), ns)
+    gen = torch.Generator().manual_seed(8)
+    ours, theirs = (gqa.new_q8_pool(30, torch.int8, dev) for _ in range(2))
+    tables = [torch.full((3, 6), -1, dtype=torch.int32, device=dev) for _ in range(2)]
+    free, n_free, cached = i32(list(range(30)), dev), i32([30], dev), i32([0, 0, 0], dev)
+    ws = gqa.new_attention_q8_workspace(3, 60, 40, dev)
+    for news in ([40, 3, 1], [1, 1, 1], [17, 2, 0]):
+        qkv = torch.randn((sum(news), 48, 128), generator=gen).to(torch.bfloat16).to(dev)
+        plan = gqa.paged_plan(cached, i32(news, dev), free, n_free, tables[0], sum(news))
+        gqa.kv_append_q8(qkv[:, 32:40], qkv[:, 40:], ours, plan.slot_map, plan.positions)
+        want = gqa.gqa_attention_q8(qkv[:, :32], ours, tables[0], plan.seq_len, plan.cu_new, max_new=max(news))
+        out, lens, left = ns["serving_step"](qkv, *theirs, tables[1], cached, i32(news, dev), free, n_free, max(news), ws)
+        assert torch.equal(out, want) and torch.equal(lens, plan.seq_len) and torch.equal(left, plan.n_free)
+        assert torch.equal(theirs.k, ours.k) and torch.equal(theirs.v_scale, ours.v_scale)
+        cached, n_free = lens, left
 
 
 def test_serving_step_graph_replays(dev):
