@@ -1,5 +1,5 @@
-// gqa_q8.h -- what the kernels of the 8-bit paged cache share: argument blocks, the two formats'
-// conversions, and one step of attention over 32 keys.
+// gqa_q8.h -- what the kernels of the 8-bit paged cache share: argument blocks and the two formats'
+// conversions.
 #pragma once
 
 #include <hip/hip_runtime.h>

@@ -37,7 +37,7 @@ constexpr float kLowest = -3.0e38f;        // a reference before any key (finite
 constexpr float kSlack = 8.0f;             // how far (log2) a key may lie above its reference
 
 // Tokens and first position of sequence b; false where it has no row to compute (lengths that
-// break the rules are the merge kernel's: NaN rows).
+// break the rules: the stream kernel gives them NaN rows).
 struct Q8Seq {
     int row0;      // its first query row
     int n;         // its rows
@@ -207,14 +207,13 @@ __device__ __forceinline__ q8_i32x2 read_v(const q8_lds* vp, uint32_t voff, int 
 
 // V of a step that some column does not see whole: rows behind `last` are cleared (they may hold
 // anything), and NaN codes, of which 0 * NaN would reach the columns that do not see their key,
-// are cleared too, after the elements of the columns that do see them have been marked.  Called by
-// all `threads` threads of the workgroup.
+// are cleared too, after the elements of the columns that do see them have been marked.  (One-wave workgroups.)
 template <int kFmt, int kTiles>
-__device__ __forceinline__ void mask_values(q8_lds* vp, int key0, int last, const int (&lim)[kTiles], int tid, int threads,
+__device__ __forceinline__ void mask_values(q8_lds* vp, int key0, int last, const int (&lim)[kTiles], int lane,
                                             Q8State<kTiles>& st) {
-    const int lane = tid & (kWave - 1), g = lane >> 4;
-    for (int row = tid >> 3; row < kQ8Step; row += threads >> 3)
-        if (key0 + row > last) *(GQA_LDS q8_u32x4*)(vp + row * kQ8RowB + 16 * (tid & 7)) = q8_u32x4{0u, 0u, 0u, 0u};
+    const int g = lane >> 4;
+    for (int row = lane >> 3; row < kQ8Step; row += kWave >> 3)
+        if (key0 + row > last) *(GQA_LDS q8_u32x4*)(vp + row * kQ8RowB + 16 * (lane & 7)) = q8_u32x4{0u, 0u, 0u, 0u};
     __syncthreads();
     if constexpr (kFmt == kQ8E4m3) {
         uint32_t any = 0;
@@ -222,7 +221,7 @@ __device__ __forceinline__ void mask_values(q8_lds* vp, int key0, int last, cons
             const q8_u32x4 w = *(GQA_LDS q8_u32x4*)(vp + row * kQ8RowB + 16 * (lane & 7));
             any |= nan_bytes(w.x) | nan_bytes(w.y) | nan_bytes(w.z) | nan_bytes(w.w);
         }
-        if (!__any(any != 0)) return;              // (the same for every wave: each looked at the whole plane)
+        if (!__any(any != 0)) return;
         const uint32_t voff = v_offset(lane);
 #pragma unroll 1
         for (int dt = 0; dt < 8; ++dt) {
@@ -244,8 +243,8 @@ __device__ __forceinline__ void mask_values(q8_lds* vp, int key0, int last, cons
             }
         }
         __syncthreads();
-        for (int row = tid >> 3; row < kQ8Step; row += threads >> 3) {
-            GQA_LDS q8_u32x4* at = (GQA_LDS q8_u32x4*)(vp + row * kQ8RowB + 16 * (tid & 7));
+        for (int row = lane >> 3; row < kQ8Step; row += kWave >> 3) {
+            GQA_LDS q8_u32x4* at = (GQA_LDS q8_u32x4*)(vp + row * kQ8RowB + 16 * (lane & 7));
             q8_u32x4 w = *at;
 #pragma unroll
             for (int i = 0; i < 4; ++i) w[i] &= ~(nan_bytes(w[i]) / 0x80u * 0xffu);
@@ -826,7 +825,7 @@ void q8_stream_kernel(Q8AttnArgs a) {
             buf = buf + 1 == kRing ? 0 : buf + 1;
             const int key0 = step * kQ8Step;
             const bool masked = key0 + kQ8Step - 1 > cur.start;
-            if (masked) mask_values<kFmt, kNow>(vp, key0, cur.start + cur.n - 1, lim, lane, kWave, st);
+            if (masked) mask_values<kFmt, kNow>(vp, key0, cur.start + cur.n - 1, lim, lane, st);
             const Q8KRows k = read_keys(kp, koff);
             float sk, lsv;
             batch_scales(batches + slot, step, lane, sk, lsv);
@@ -954,7 +953,7 @@ __device__ void find_tile(const Q8AttnArgs& a, int x, int lane, int& b, int& i) 
 }
 
 // Runs that each tile's keys are cut into: as many as the workgroups can take at once.
-__device__ __forceinline__ int tile_runs(int tiles, int wgs) { return max(1, wgs / max(1, tiles * kHkv)); }
+__device__ __forceinline__ int tile_runs(int tiles, int wgs) { return max(1, wgs / (max(1, min(tiles, wgs)) * kHkv)); }
 
 // Steps of a run of a tile of `steps` steps.
 __device__ __forceinline__ int run_steps(int steps, int runs) { return max(kTileMinRun, (steps + runs - 1) / runs); }
