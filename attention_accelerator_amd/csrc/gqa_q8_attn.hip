@@ -912,7 +912,7 @@ constexpr int kTileWaves = 8;
 constexpr int kTileCols = kQ8TileTokens * kGroup;
 constexpr int kTileRowB = 2 * kD;          // bytes of a row in fp16
 constexpr int kTilePlaneB = kQ8Step * kTileRowB;       // K (or V) of a step in fp16
-constexpr int kTileMinRun = 8;             // steps of the shortest run
+constexpr int kTileMinRun = 4;             // steps of the shortest run (40 tokens over 1000: 24 us, of 8: 28)
 
 namespace {
 
