@@ -620,7 +620,7 @@ __device__ __forceinline__ void merge_token(const Q8AttnArgs& a, int n, RowOf ro
 // The eight waves of a range are neighbours, one on each XCD, and read the eight heads' parts of the
 // same blocks at about the same time: HBM sees blocks of 16 KB, not 2.
 //
-// HBM bounds it: 64 sequences of 512..8192 keys, 661 MB, take 111 us, 6.0 TB/s; 8 of 131072, 2.16 GB, 336,
+// HBM bounds it: 64 sequences of 512..8192 keys, 661 MB, take 112 us, 5.9 TB/s; 8 of 131072, 2.16 GB, 338,
 // 6.4 TB/s.  One wave reads a step's eight operands together, before its arithmetic (left in place, each
 // waits for LDS: 113 -> 122 us for 8 tokens a sequence).  A single sequence of 4096 keys takes 13 us, its
 // ranges 4 steps long: a chain of lengths, ids, scales and keys, and the merge's.
@@ -903,7 +903,7 @@ void q8_stream_kernel(Q8AttnArgs a) {
 // where both convert at the end: 308).  Where the tiles do not fill the workgroups their keys are cut
 // into runs.
 //
-// 4 sequences with chunks of 512 tokens over 8192 take 303 us: 937 TFLOP/s of products.  A step of 32 keys
+// 4 sequences with chunks of 512 tokens over 8192 take 306 us: 928 TFLOP/s of products.  A step of 32 keys
 // takes a SIMD 2350 clocks: 1024 of products, about 1600 of vector issue (exponentials, sums, conversions), 1024
 // of the CU's LDS reads; the two waves overlap them only in part.  (Codes in LDS that every wave converts for
 // itself: 348 us; only V as codes: 337; four waves of four column tiles, a SIMD each: 480; the second wave
