@@ -118,7 +118,8 @@ def paged_plan(cached: torch.Tensor, n_new: torch.Tensor, free_blocks: torch.Ten
     if out is None:
         if n_rows < 0 or batch == 0:
             check(_lib.GQA_ERR_INVALID_CONFIG, "gqa_paged_plan")
-        out = PagedPlan(*torch.empty(sum(sizes), dtype=torch.int32, device=device).split_with_sizes(sizes))
+        # (one allocation; the unsafe split keeps no record for autograd, which integers have no use for)
+        out = PagedPlan(*torch.empty(sum(sizes), dtype=torch.int32, device=device).unsafe_split_with_sizes(sizes))
     else:
         inputs = [_span(t) for t in (cached, n_new, free_blocks, n_free, block_table)]
         for t, n, name in zip(out, sizes, PagedPlan._fields):
