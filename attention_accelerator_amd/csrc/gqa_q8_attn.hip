@@ -37,7 +37,7 @@ constexpr float kLowest = -3.0e38f;        // a reference before any key (finite
 constexpr float kSlack = 8.0f;             // how far (log2) a key may lie above its reference
 
 // Tokens and first position of sequence b; false where it has no row to compute (lengths that
-// break the rules: the stream kernel gives them NaN rows).
+// break the rules: NaN rows, by the launch that merges).
 struct Q8Seq {
     int row0;      // its first query row
     int n;         // its rows
@@ -492,13 +492,18 @@ struct Q8Shared {
     }
 };
 
-// NaN rows (of KV head h) for a sequence whose lengths break the rules, or that has more than max_new
-// rows; none where its offsets do.
-__device__ __forceinline__ void write_nan(const Q8AttnArgs& a, const Q8Seq& sq, int h, int lane) {
-    if (sq.row0 < 0 || sq.n <= 0 || static_cast<int64_t>(sq.row0) + sq.n > a.n_tokens) return;
-    for (int t = 0; t < sq.n; ++t) {
-        uint32_t* row = reinterpret_cast<uint32_t*>(a.out) + ((static_cast<int64_t>(sq.row0) + t) * kHq + kGroup * h) * (kD / 2);
-        for (int i = lane; i < kGroup * kD / 2; i += kWave) row[i] = 0x7fc07fc0u;
+// NaN rows (of KV head h) for the window's sequences whose lengths break the rules, or that have more than
+// max_new rows; none where their offsets do.  By `parts` waves, which deal the rows out; this is wave `part`.
+__device__ __forceinline__ void write_nans(const Q8AttnArgs& a, const Q8Window& win, int h, int lane, int part, int parts) {
+    for (uint64_t bad = __ballot(win.bad); bad; bad &= bad - 1) {
+        const int at = __builtin_ctzll(bad);
+        const int row0 = lane_value(win.seq.row0, at), n = lane_value(win.seq.n, at);
+        if (row0 < 0 || static_cast<int64_t>(row0) + n > a.n_tokens) continue;
+        for (int t = (part + at) % parts; t < n; t += parts) {
+            uint16_t* row = a.out + ((static_cast<int64_t>(row0) + t) * kHq + kGroup * h) * kD + 4 * lane;
+            *reinterpret_cast<uint2*>(row) = make_uint2(0x7fc07fc0u, 0x7fc07fc0u);
+            *reinterpret_cast<uint2*>(row + kGroup * kD / 2) = make_uint2(0x7fc07fc0u, 0x7fc07fc0u);
+        }
     }
 }
 
@@ -647,11 +652,7 @@ void q8_stream_kernel(Q8AttnArgs a) {
         win.load(a, b0, lane);
         all += static_cast<uint32_t>(lane_value(wave_scan(win.steps), kWave - 1));
         seqs += __popcll(__ballot(win.steps > 0));
-        for (uint64_t bad = __ballot(win.bad); bad; bad &= bad - 1) {      // the wave of (b, h): b by the ranges in turn
-            const int at = __builtin_ctzll(bad);
-            if ((b0 + at) % (a.stream_waves / kHkv) != wave / kHkv) continue;
-            write_nan(a, Q8Seq{lane_value(win.seq.row0, at), lane_value(win.seq.n, at), 0}, h, lane);
-        }
+        if constexpr (kOne) write_nans(a, win, h, lane, wave / kHkv, a.stream_waves / kHkv);
     }
     // (all lanes store the same: under a branch on the lane the compiler keeps the loop's uniform values in
     // vector registers, 32 more)
@@ -1226,6 +1227,15 @@ __global__ __launch_bounds__(kWave) void q8_merge_kernel(Q8AttnArgs a, int cols,
     }
     const int first = blockIdx.x / kHkv % waves, r0 = blockIdx.x / kHkv / waves;
     const Q8CutSeq seq = a.cut_seqs[r0];
+    if (first == 0) {                              // the windows of sequences dealt over the ranges, or the ranges over them
+        const int ranges = a.stream_waves / kHkv, windows = (a.batch + kWave - 1) / kWave;
+        const int parts = max(1, ranges / windows), part = r0 / windows;
+        for (int w = r0 % windows; w < windows && part < parts; w += ranges) {
+            Q8Window win;
+            win.load(a, w * kWave, lane);
+            write_nans(a, win, h, lane, part, parts);
+        }
+    }
     if (first >= seq.n) return;
     const int pieces = 1 + static_cast<int>((seq.left + seq.per - 1) / seq.per);
     for (int tok = first; tok < seq.n; tok += waves) {

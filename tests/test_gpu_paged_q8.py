@@ -504,6 +504,20 @@ def test_attention_many_sequences(dev, most):
     assert_close(got[keep], want[keep], bound[keep], str(most))
 
 
+@pytest.mark.parametrize("most", [1, 700])
+def test_attention_refused_sequences(dev, most):
+    """Refused sequences (length 0) of one and of many rows between others: NaN rows, all of them, and no other."""
+    news = [most, 1, most, 1, 1] if most > 1 else [1] * 200
+    lens = [0, 40, 0, 0, 25] if most > 1 else [33 * (b % 3 == 1) for b in range(200)]
+    q, pool, table, cu = make_batch("int8", news, [max(n, m) for n, m in zip(news, lens)], seed=most)
+    out = torch.full((cu[-1] + 2, 32, 128), 5.0, dtype=torch.bfloat16, device=dev)
+    q = torch.cat((q, q[:2]))
+    gqa.gqa_attention_q8(q.to(dev), to_dev(pool, dev), i32(table, dev), i32(lens, dev), i32(cu, dev), max_new=most, out=out)
+    for b, n in enumerate(lens):
+        assert out[cu[b]:cu[b + 1]].isnan().all() if n == 0 else out[cu[b]:cu[b + 1]].isfinite().all(), b
+    assert (out[cu[-1]:] == 5).all()
+
+
 def test_attention_one_workspace_for_all(dev):
     """Calls of every kind in turn on one workspace, and rows behind the last sequence."""
     batches = [([1, 1, 1], [700, 40, 1300]), ([40, 1], [900, 33]), ([8, 3], [500, 777]), ([1], [3000]), ([1] * 70, [90] * 70)]
